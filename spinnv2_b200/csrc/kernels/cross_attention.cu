@@ -1,0 +1,234 @@
+// Attention of queries to an encoder's keys and values of another length:
+//
+//   o_i = sum_j p_ij v_j,  p_i = softmax over the keys that count of scale <q_i, k_j>
+//
+// No causal order, so the queries of one entry and all the query heads that
+// share a key head attend to the same keys: they are laid out as one list of
+// rows, r = query * group + (head in the group), and a tile of rows reads
+// each key and value once for all of them.
+//
+// The keys pass once, in tiles, with each row's running maximum m and sum l:
+// a tile's scores raise m to m', the sums so far shrink by exp(m - m'), and
+// the result is divided by l at the end.  Exponents are taken in base 2, with
+// scale * log2(e) as the factor.  A key that does not count has score -inf and
+// is read as zeros, so that what lies there (NaN included) has no influence;
+// a row without keys keeps l = 0 and is written as 0.
+#include "transformer.cuh"
+
+namespace spkv2 {
+
+namespace {
+
+using namespace xf;
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void *out;
+  const int32_t *lengths;
+  const uint8_t *key_mask;
+  int64_t qs[3], ks[3], vs[3], os[3];  // batch, token, head
+  int64_t mask_stride;
+  int batch, queries, keys, kv_heads, group, width;
+  int rows;        // queries * group
+  int row_tiles;   // per (batch, key head)
+  float scale_log2;
+};
+
+__device__ __forceinline__ int entry_keys(const AttnArgs &p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
+}
+
+// ------------------------------------------------------------ CUDA cores
+// Any type, width and alignment, exact fp32 products.  64 rows x 64 keys a
+// step, 256 threads; a thread holds scores for 4 rows x 4 keys and sums for
+// 4 rows x D / 16 columns.  The 16 threads of a row group are half a warp.
+constexpr int kRows = 64, kKeys = 64;
+
+template <int D>
+struct SimtSmem {
+  float q[kRows][D + 4];
+  float k[kKeys][D + 4];
+  float v[kKeys][D];
+  float p[kRows][kKeys + 4];
+  int valid[kKeys];
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SimtSmem<D> &sm = *reinterpret_cast<SimtSmem<D> *>(smem_raw);
+  constexpr int CPT = D / 16;  // columns of a thread: tx * CW + 16 * CW * c
+  constexpr int CW = CPT < 4 ? CPT : 4;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  int t = blockIdx.x;
+  const int r0 = t % a.row_tiles * kRows;
+  t /= a.row_tiles;
+  const int hk = t % a.kv_heads, b = t / a.kv_heads;
+  const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
+  const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
+  const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
+  const int keys = entry_keys(a, b);
+
+  for (int e = tid; e < kRows * D; e += 256) {
+    const int r = e / D, c = e % D, row = r0 + r;
+    float val = 0.0f;
+    if (row < a.rows && c < a.width) {
+      const int qi = row / a.group, h = hk * a.group + row % a.group;
+      val = to_f32(q[qi * a.qs[1] + h * a.qs[2] + c]);
+    }
+    sm.q[r][c] = val;
+  }
+  float o[4][CPT] = {}, m[4], l[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
+
+  for (int j0 = 0; j0 < keys; j0 += kKeys) {
+    __syncthreads();  // the last tile's readers are done
+    if (tid < kKeys) {
+      const int j = j0 + tid;
+      sm.valid[tid] = j < keys && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
+    }
+    __syncthreads();
+    for (int e = tid; e < kKeys * D; e += 256) {
+      const int r = e / D, c = e % D;
+      const bool in = sm.valid[r] && c < a.width;
+      sm.k[r][c] = in ? to_f32(k[(j0 + r) * a.ks[1] + c]) : 0.0f;
+      sm.v[r][c] = in ? to_f32(v[(j0 + r) * a.vs[1] + c]) : 0.0f;
+    }
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 4
+    for (int c = 0; c < D; c += 4) {
+      float4 qv[4], kv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qv[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * 4 + i][c]);
+        kv[i] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * i][c]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
+          s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
+          s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
+          s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = sm.valid[tx + 16 * j] ? s[i][j] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int w = 8; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      const float use = mx == -INFINITY ? 0.0f : mx;
+      const float shrink = exp2f(m[i] - use);
+      m[i] = mx;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(s[i][j] - use);
+        sum += e;
+        sm.p[ty * 4 + i][tx + 16 * j] = e;
+      }
+      l[i] = l[i] * shrink + sum;  // this thread's keys only; joined at the end
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) o[i][c] *= shrink;
+    }
+    __syncwarp();  // a row's 16 threads are in one warp
+#pragma unroll 2
+    for (int j = 0; j < kKeys; j += 4) {
+      float4 pv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4 *>(&sm.p[ty * 4 + i][j]);
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+#pragma unroll
+        for (int c = 0; c < CPT; c += CW) {
+          float vv[CW];
+#pragma unroll
+          for (int w = 0; w < CW; ++w) vv[w] = sm.v[j + jj][tx * CW + 16 * c + w];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w;
+#pragma unroll
+            for (int w = 0; w < CW; ++w) o[i][c + w] = fmaf(e, vv[w], o[i][c + w]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sum = l[i];
+#pragma unroll
+    for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    const int row = r0 + ty * 4 + i;
+    if (row >= a.rows) continue;
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const int qi = row / a.group, h = hk * a.group + row % a.group;
+    T *out = static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+      const int col = tx * CW + 16 * (c / CW * CW) + c % CW;
+      if (col < a.width) out[col] = from_f32<T>(o[i][c] * inv);
+    }
+  }
+}
+
+template <class T, int D>
+int launch_simt(AttnArgs a, cudaStream_t s) {
+  a.row_tiles = int(ceil_div(a.rows, kRows));
+  const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
+  if (blocks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  auto kern = cross_simt_kernel<T, D>;
+  const int rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SimtSmem<D>)));
+  if (rc) return rc;
+  kern<<<unsigned(blocks), 256, sizeof(SimtSmem<D>), s>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+}  // namespace spkv2
+
+using namespace spkv2;
+using namespace spkv2::xf;
+
+extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *stream) {
+  if (!x || x->batch < 0 || x->queries < 0 || x->keys < 0 || x->kv_heads < 1 || x->heads < 1 ||
+      x->heads % x->kv_heads != 0 || x->width < 1)
+    return -1;
+  if (x->batch == 0 || x->queries == 0) return 0;
+  if (!x->q || !x->out || (x->keys > 0 && (!x->k || !x->v))) return -1;
+  for (int i = 0; i < 3; ++i)
+    if (x->q_stride[i] < 0 || x->k_stride[i] < 0 || x->v_stride[i] < 0 || x->out_stride[i] < 0) return -1;
+  if (x->key_mask && x->mask_stride < 0) return -1;
+  if (!isfinite(x->scale)) return -1;
+  const int group = x->heads / x->kv_heads;
+  if (!elem_bytes(x->dtype) || x->width > 256 || x->batch > INT32_MAX || x->keys > INT32_MAX - 1024 ||
+      x->queries > (INT32_MAX - 1024) / group)
+    return SPKV2_ERR_UNSUPPORTED;
+  AttnArgs a = {};
+  a.q = x->q, a.k = x->k, a.v = x->v, a.out = x->out, a.lengths = x->lengths, a.key_mask = x->key_mask;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = x->q_stride[i], a.ks[i] = x->k_stride[i], a.vs[i] = x->v_stride[i], a.os[i] = x->out_stride[i];
+  }
+  a.mask_stride = x->mask_stride;
+  a.batch = int(x->batch), a.queries = int(x->queries), a.keys = int(x->keys);
+  a.kv_heads = x->kv_heads, a.group = group, a.width = x->width;
+  a.rows = a.queries * group;
+  a.scale_log2 = x->scale * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_type(x->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (a.width <= 32) return launch_simt<T, 32>(a, s);
+    if (a.width <= 64) return launch_simt<T, 64>(a, s);
+    if (a.width <= 128) return launch_simt<T, 128>(a, s);
+    return launch_simt<T, 256>(a, s);
+  });
+}
