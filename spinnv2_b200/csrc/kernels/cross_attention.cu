@@ -185,10 +185,8 @@ int launch_simt(AttnArgs a, cudaStream_t s) {
   a.row_tiles = int(ceil_div(a.rows, kRows));
   const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
   if (blocks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  auto kern = cross_simt_kernel<T, D>;
-  const int rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SimtSmem<D>)));
-  if (rc) return rc;
-  kern<<<unsigned(blocks), 256, sizeof(SimtSmem<D>), s>>>(a);
+  if (const int rc = allow_smem<cross_simt_kernel<T, D>>(sizeof(SimtSmem<D>))) return rc;
+  cross_simt_kernel<T, D><<<unsigned(blocks), 256, sizeof(SimtSmem<D>), s>>>(a);
   return cuda_status(cudaGetLastError());
 }
 

@@ -3,6 +3,7 @@
 //   y[i, j] = act(float(sum_k a[i, k] w[j, k]) * a_scale[i] * w_scale[j] + bias[j])
 //
 // The sum is exact in int32 (|a|, |w| <= 128 and k <= 131071).
+#include "tcgen05.cuh"
 #include "transformer.cuh"
 
 namespace spkv2 {
@@ -10,6 +11,7 @@ namespace spkv2 {
 namespace {
 
 using namespace xf;
+using namespace tc;
 
 constexpr int64_t kMaxK = 131071;  // 128 * 128 * k stays below 2^31
 
@@ -75,6 +77,395 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(LinearArgs p) {
   }
 }
 
+// ------------------------------------------------------------ tensor cores
+// Both kernels compute the transposed tile: the 128 rows of an MMA are output
+// CHANNELS (weight rows) and its columns are tokens.  A TMEM lane is then a
+// channel, so a thread keeps its channel's scale and bias in registers, the 32
+// lanes of a warp store 32 neighbouring channels of one token, and a few
+// tokens cost a few columns, not 128 rows.  K steps are 128 bytes, four MMAs
+// of K = 32; TMA fills what lies beyond k, n and m with zeros.
+constexpr int kBP = 128;                 // channels of a CTA's tile
+constexpr int kBK = 128;                 // int8 elements of a K step
+constexpr int kPBytes = kBP * kBK;
+
+__device__ int g_linear_status;  // role code of the last bounded wait that gave up
+
+// Codes of the bounded waits: 2 TMA producer, 3 MMA issuer, 4 epilogue, 5
+// landing relay, 7 accumulator hand-off.
+
+// The TMA loads issued into a ring of stages have landed (a bounded wait each,
+// at most the last `stages` of `issued`): shared memory must not go away first.
+__device__ __forceinline__ void drain_loads(uint64_t *full_bar, int stages, uint32_t issued) {
+  for (uint32_t it = issued > uint32_t(stages) ? issued - uint32_t(stages) : 0; it < issued; ++it) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(&full_bar[it % uint32_t(stages)], (it / uint32_t(stages)) & 1) && clock64() - t0 < kWaitCycles) {
+    }
+  }
+}
+
+// A chunk of COLS (at most 32) accumulator columns: tokens m, m + 1, .. of this
+// thread's channel.
+template <class T, int COLS>
+__device__ __forceinline__ void store_chunk(const LinearArgs &p, const uint32_t (&acc)[32], int64_t n, int64_t m, int lane,
+                                            float sw, float bias) {
+  const float mine = m + lane < p.m ? __ldg(p.a_scale + m + lane) : 0.0f;
+  const int cnt = int(min(int64_t(COLS), p.m - m));
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = fmaf(float(int(acc[j])) * __shfl_sync(0xffffffffu, mine, j), sw, bias);
+  apply_act32(v, p.act);
+  if (n >= p.n) return;
+  T *y = static_cast<T *>(p.y) + m * p.y_stride + n;
+#pragma unroll
+  for (int j = 0; j < COLS; ++j)
+    if (j < cnt) y[j * p.y_stride] = from_f32<T>(v[j]);
+}
+
+// Few tiles: one tile of 128 channels x BN tokens per cluster, whose CTAs
+// divide k.  Each CTA leaves its int32 sums in its own shared memory and
+// takes BN / cluster columns of everybody's: integer sums, so the order does
+// not matter, and nothing passes through global memory.  Warps 0-3 epilogue,
+// 4 TMA producer, 5 MMA.
+constexpr int kSplitThreads = 192;
+constexpr int split_stages(int bn) { return bn >= 256 ? 4 : bn == 128 ? 6 : bn == 64 ? 8 : 10; }
+constexpr size_t split_smem(int bn) { return size_t(split_stages(bn)) * (kPBytes + bn * kBK) + 1024; }
+
+template <class T, int BN>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    linear_split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap, LinearArgs p,
+                        int n_tiles, int num_kb, int csize) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int STAGES = split_stages(BN);
+  constexpr int STAGE = kPBytes + BN * kBK;
+  constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
+  static_assert(STAGES * STAGE >= BN * kBP * 4, "the partial sums reuse the operand stages");
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int abort_flag;
+  int *status = &g_linear_status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = csize > 1 ? int(cluster_rank()) : 0;
+  const int tile = int(blockIdx.x) / csize;
+  const int64_t n0 = int64_t(tile % n_tiles) * kBP, m0 = int64_t(tile / n_tiles) * BN;
+  const int kb0 = int(int64_t(num_kb) * rank / csize), kb1 = int(int64_t(num_kb) * (rank + 1) / csize);
+
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&acc_bar, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const uint32_t trow = tmem + (uint32_t(warp * 32) << 16);
+  const int64_t n = n0 + warp * 32 + lane;  // warps 0-3
+  int32_t *part = reinterpret_cast<int32_t *>(smem);  // [column][channel]
+  bool landed = false;
+  if (warp < 4) {
+    landed = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0, &abort_flag, status, 4));
+    tc_fence_after();
+    if (landed && csize == 1) {
+      const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
+      const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        if (m0 + c >= p.m) break;
+        uint32_t acc[32];
+        tmem_ld32(trow + uint32_t(c), acc);
+        store_chunk<T, BN < 32 ? BN : 32>(p, acc, n, m0 + c, lane, sw, bias);
+      }
+    } else if (landed) {
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t acc[32];
+        tmem_ld32(trow + uint32_t(c), acc);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < BN) part[(c + j) * kBP + warp * 32 + lane] = int32_t(acc[j]);
+      }
+    }
+  } else if (warp == 4) {
+    if (lane == 0) {
+      int it = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, &abort_flag, status, 2)) break;
+        uint8_t *st = smem + s * STAGE;
+        mbar_arrive_expect_tx(&full_bar[s], STAGE);
+        tma_load_2d(st, &wmap, kb * kBK, int(n0), &full_bar[s]);
+        tma_load_2d(st + kPBytes, &amap, kb * kBK, int(m0), &full_bar[s]);
+      }
+      drain_loads(full_bar, STAGES, uint32_t(it));
+    }
+  } else if (lane == 0) {
+    constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBP >> 4) << 24);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int it = kb - kb0, s = it % STAGES;
+      if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, &abort_flag, status, 3)) break;
+      tc_fence_after();
+      const uint64_t da = smem_desc(smem + s * STAGE), db = smem_desc(smem + s * STAGE + kPBytes);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        mma_i8(tmem, da + kk * 2, db + kk * 2, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+      mma_commit(&empty_bar[s]);
+    }
+    mma_commit(&acc_bar);  // completes once every MMA issued above has
+  }
+  __syncwarp();
+  if (csize > 1) {
+    cluster_sync();
+    if (warp < 4 && !abort_flag) {
+      const int per = BN / csize;
+      const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
+      const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+#pragma unroll 1
+      for (int c = rank * per; c < (rank + 1) * per; ++c) {
+        const int64_t m = m0 + c;
+        if (m >= p.m) break;
+        const int32_t *own = part + c * kBP + warp * 32 + lane;
+        int sum = 0;
+        for (int r = 0; r < csize; ++r) sum += int(ld_cluster(map_rank(own, uint32_t(r))));
+        if (n < p.n)
+          static_cast<T *>(p.y)[m * p.y_stride + n] = from_f32<T>(linear_value(sum, __ldg(p.a_scale + m), sw, bias, p.act));
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // the peers have read this CTA's sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    if (lane == 0) {  // every issued MMA has finished before TMEM is freed (also after a wait that gave up)
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&acc_bar, 0) && clock64() - t0 < kWaitCycles) {
+      }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// Many tiles: persistent CTA pairs, tiles of 256 channels x 256 tokens.  Each
+// CTA holds its 128 channels and 128 of the tokens, so a K step brings it 32 KB
+// for 256 x 256 x 128 products (a lone CTA would need 48 KB for half of them,
+// more than L2 can give every SM).  Two accumulator buffers in TMEM: a tile's
+// epilogue runs under the next tile's MMAs.  Warps 0-7 epilogue, 8 TMA
+// producer, 9 MMA (in the leader) or landing relay (in its peer).
+constexpr int kPairThreads = 320, kPairN = 256, kPairStages = 6;
+constexpr int kPairStage = kPBytes + kPairN / 2 * kBK;
+constexpr size_t kPairSmem = size_t(kPairStages) * kPairStage + 1024;
+
+template <class T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap, LinearArgs p,
+                       int n_tiles, int tiles, int num_kb) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[kPairStages], peer_bar[kPairStages], empty_bar[kPairStages], accf_bar[2], acce_bar[2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int abort_flag;
+  int *status = &g_linear_status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = int(cluster_rank());
+  const int tile0 = int(cluster_id_x()), tstep = int(cluster_count_x());
+  const int my_tiles = tile0 < tiles ? (tiles - 1 - tile0) / tstep + 1 : 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full_bar[s], 1);   // this CTA's operands have landed
+      mbar_init(&peer_bar[s], 1);   // (leader) the peer's have
+      mbar_init(&empty_bar[s], 1);  // the leader's MMAs have read the stage
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf_bar[b], 1);
+      mbar_init(&acce_bar[b], 16);  // one arrival per epilogue warp of both CTAs
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp < 8) {
+    const int quarter = warp & 3, col0 = (warp >> 2) * (kPairN / 2);
+    for (int ti = 0; ti < my_tiles; ++ti) {
+      const int t = tile0 + ti * tstep, ab = ti & 1;
+      const int64_t n = int64_t(t % n_tiles) * 2 * kBP + rank * kBP + quarter * 32 + lane;
+      const int64_t m0 = int64_t(t / n_tiles) * kPairN;
+      const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
+      const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+      if (!__all_sync(0xffffffffu, mbar_wait_cluster(&accf_bar[ab], (ti >> 1) & 1, &abort_flag, status, 4))) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = col0; c < col0 + kPairN / 2; c += 32) {
+        uint32_t acc[32];
+        tmem_ld32(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(ab * kPairN + c), acc);
+        if (c + 32 == col0 + kPairN / 2) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_rank(&acce_bar[ab], 0);
+        }
+        if (m0 + c < p.m) store_chunk<T, 32>(p, acc, n, m0 + c, lane, sw, bias);
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int ti = 0; ti < my_tiles && ok; ++ti) {
+        const int t = tile0 + ti * tstep;
+        const int n0 = t % n_tiles * 2 * kBP + rank * kBP, m0 = t / n_tiles * kPairN + rank * (kPairN / 2);
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % kPairStages;
+          ok = mbar_wait_cluster(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, &abort_flag, status, 2);
+          if (!ok) break;
+          uint8_t *st = smem + s * kPairStage;
+          mbar_arrive_expect_tx(&full_bar[s], kPairStage);
+          tma_load_2d(st, &wmap, kb * kBK, n0, &full_bar[s]);
+          tma_load_2d(st + kPBytes, &amap, kb * kBK, m0, &full_bar[s]);
+        }
+      }
+      drain_loads(full_bar, kPairStages, it);
+    }
+  } else if (lane == 0 && rank == 1) {
+    const uint32_t total = uint32_t(my_tiles) * uint32_t(num_kb);
+    for (uint32_t it = 0; it < total; ++it) {
+      const int s = it % kPairStages;
+      if (!mbar_wait(&full_bar[s], (it / kPairStages) & 1, &abort_flag, status, 5)) break;
+      mbar_arrive_rank(&peer_bar[s], 0);
+    }
+    // The leader's last MMAs end before this CTA frees its half of TMEM: the
+    // cluster barrier below, which the leader reaches after its last commit.
+  } else if (lane == 0) {
+    constexpr uint32_t idesc =
+        (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairN >> 3) << 17) | (uint32_t(2 * kBP >> 4) << 24);
+    uint32_t it = 0;
+    int done = 0;
+    bool ok = true;
+    for (int ti = 0; ti < my_tiles && ok; ++ti) {
+      const int ab = ti & 1;
+      ok = mbar_wait_cluster(&acce_bar[ab], ((ti >> 1) & 1) ^ 1, &abort_flag, status, 7);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < num_kb; ++kb, ++it) {
+        const int s = it % kPairStages;
+        const uint32_t ph = (it / kPairStages) & 1;
+        ok = mbar_wait(&full_bar[s], ph, &abort_flag, status, 3) && mbar_wait_cluster(&peer_bar[s], ph, &abort_flag, status, 3);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t da = smem_desc(smem + s * kPairStage), db = smem_desc(smem + s * kPairStage + kPBytes);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_i8_pair(tmem + uint32_t(ab * kPairN), da + kk * 2, db + kk * 2, idesc, (kb | kk) ? 1u : 0u);
+        mma_commit_pair(&empty_bar[s]);
+      }
+      if (!ok) break;
+      mma_commit_pair(&accf_bar[ab]);
+      ++done;
+    }
+    if (done > 0) {  // every issued MMA has finished before TMEM is freed
+      const long long t0 = clock64();
+      while (!mbar_try_wait_cluster(&accf_bar[(done - 1) & 1], ((done - 1) >> 1) & 1) && clock64() - t0 < kWaitCycles) {
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();  // the leader's MMAs read the peer's shared memory until here
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ------------------------------------------------------------ choice
+// TMA reads rows that start on 16-byte boundaries.
+bool tma_rows(const int8_t *base, int64_t rows, int64_t stride, int k) {
+  return aligned16(base) && (rows == 1 || (stride % 16 == 0 && stride >= k));
+}
+
+bool encode_rows(CUtensorMap *map, const int8_t *base, int64_t rows, int64_t stride, int k, int box) {
+  const uint64_t pitch = rows == 1 ? (uint64_t(k) + 15) / 16 * 16 : uint64_t(stride);
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, uint64_t(k), uint64_t(rows), pitch, uint32_t(box));
+}
+
+template <class T, int BN>
+int launch_split(const LinearArgs &p, int n_tiles, int m_tiles, int num_kb, int csize, cudaStream_t s) {
+  if (const int rc = allow_smem<linear_split_kernel<T, BN>>(split_smem(BN))) return rc;
+  CUtensorMap wmap, amap;
+  if (!encode_rows(&wmap, p.w, p.n, p.w_stride, p.k, kBP) || !encode_rows(&amap, p.a, p.m, p.a_stride, p.k, BN))
+    return SPKV2_ERR_CUDA;
+  return cuda_status(launch_kernel(linear_split_kernel<T, BN>, unsigned(n_tiles * m_tiles * csize), kSplitThreads, split_smem(BN), s, csize, wmap,
+                                   amap, p, n_tiles, num_kb, csize));
+}
+
+template <class T>
+int launch_pair(const LinearArgs &p, int n_tiles, int m_tiles, int num_kb, cudaStream_t s) {
+  if (const int rc = allow_smem<linear_pair_kernel<T>>(kPairSmem)) return rc;
+  CUtensorMap wmap, amap;
+  if (!encode_rows(&wmap, p.w, p.n, p.w_stride, p.k, kBP) || !encode_rows(&amap, p.a, p.m, p.a_stride, p.k, kPairN / 2))
+    return SPKV2_ERR_CUDA;
+  const int tiles = n_tiles * m_tiles;
+  return cuda_status(launch_kernel(linear_pair_kernel<T>, 2u * unsigned(std::min(tiles, sm_count() / 2)), kPairThreads, kPairSmem, s, 2, wmap,
+                                   amap, p, n_tiles, tiles, num_kb));
+}
+
+// The cheapest shape by the cycles of its busiest SM: MMA steps (2 cycles for
+// each token column of a K step) or operand bytes (64 a cycle from L2),
+// whichever is more, times the tiles it runs one after another.
+template <class T>
+int launch_tc(const LinearArgs &p, cudaStream_t s) {
+  const int num_kb = int(ceil_div(p.k, kBK)), sms = sm_count();
+  const int64_t n_tiles = ceil_div(p.n, kBP);
+  int best_bn = 0, best_c = 1;
+  double best = 1e30;
+  for (int bn = 16; bn <= 256; bn *= 2) {
+    const int64_t tiles = n_tiles * ceil_div(p.m, bn);
+    if (tiles > INT32_MAX / 8) continue;
+    for (int c = 1; c <= 8; c *= 2) {
+      if (c > 1 && (num_kb < 2 * c || tiles * c > sms)) break;
+      const double step = std::max(2.0 * bn, (kBP + bn) * kBK / 64.0);
+      const double cost = double(ceil_div(tiles * c, sms)) * (1500.0 + ceil_div(num_kb, c) * step + 6.0 * bn) + (c > 1 ? 1000.0 : 0.0);
+      if (cost < best) best = cost, best_bn = bn, best_c = c;
+    }
+  }
+  const int64_t pn = ceil_div(p.n, 2 * kBP), pm = ceil_div(p.m, kPairN);
+  const double pair = double(ceil_div(pn * pm, sms / 2)) * num_kb * 512.0 + 4000.0;
+  if (pn * pm <= INT32_MAX / 2 && (pair < best || !best_bn)) return launch_pair<T>(p, int(pn), int(pm), num_kb, s);
+  const int nt = int(n_tiles), mt = int(ceil_div(p.m, best_bn));
+  switch (best_bn) {
+    case 16: return launch_split<T, 16>(p, nt, mt, num_kb, best_c, s);
+    case 32: return launch_split<T, 32>(p, nt, mt, num_kb, best_c, s);
+    case 64: return launch_split<T, 64>(p, nt, mt, num_kb, best_c, s);
+    case 128: return launch_split<T, 128>(p, nt, mt, num_kb, best_c, s);
+    default: return launch_split<T, 256>(p, nt, mt, num_kb, best_c, s);
+  }
+}
+
 }  // namespace
 
 }  // namespace spkv2
@@ -93,9 +484,12 @@ extern "C" int spkv2_cuda_linear_i8(const Spkv2LinearI8 *a, void *stream) {
                         a->y_stride, int(a->k), a->activation};
   const int64_t tiles = ceil_div(a->m, kST) * ceil_div(a->n, kST);
   if (tiles > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.k > 0 && tma_rows(p.a, p.m, p.a_stride, p.k) && tma_rows(p.w, p.n, p.w_stride, p.k) && encode_fn())
+    return by_type(a->dtype, [&](auto t) { return launch_tc<decltype(t)>(p, s); });
   return by_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    linear_simt_kernel<T><<<unsigned(tiles), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    linear_simt_kernel<T><<<unsigned(tiles), 256, 0, s>>>(p);
     return cuda_status(cudaGetLastError());
   });
 }

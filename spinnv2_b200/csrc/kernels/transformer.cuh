@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "spkv2_transformer.h"
 
 #include "common.cuh"
@@ -63,6 +65,20 @@ inline int sm_count() {
     return v;
   }();
   return n;
+}
+
+// Lets KERN use `bytes` of dynamic shared memory on the current device; asked
+// of the driver once for each device.
+template <auto KERN>
+inline int allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return SPKV2_ERR_NO_DEVICE;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  const cudaError_t err = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return cuda_status(err);
 }
 
 }  // namespace xf
