@@ -90,8 +90,8 @@ constexpr int kPBytes = kBP * kBK;
 
 __device__ int g_linear_status;  // role code of the last bounded wait that gave up
 
-// Codes of the bounded waits: 2 TMA producer, 3 MMA issuer, 4 epilogue, 5
-// landing relay, 7 accumulator hand-off.
+// Codes of the bounded waits: 2 TMA producer, 3 MMA issuer, 4 epilogue, 7
+// accumulator hand-off.
 
 // The TMA loads issued into a ring of stages have landed (a bounded wait each,
 // at most the last `stages` of `issued`): shared memory must not go away first.
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // for 256 x 256 x 128 products (a lone CTA would need 48 KB for half of them,
 // more than L2 can give every SM).  Two accumulator buffers in TMEM: a tile's
 // epilogue runs under the next tile's MMAs.  Warps 0-7 epilogue, 8 TMA
-// producer, 9 MMA (in the leader) or landing relay (in its peer).
+// producer, 9 MMA (in the leader).
 constexpr int kPairThreads = 320, kPairN = 256, kPairStages = 6;
 constexpr int kPairStage = kPBytes + kPairN / 2 * kBK;
 constexpr size_t kPairSmem = size_t(kPairStages) * kPairStage + 1024;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                        int n_tiles, int tiles, int num_kb) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full_bar[kPairStages], peer_bar[kPairStages], empty_bar[kPairStages], accf_bar[2], acce_bar[2];
+  __shared__ uint64_t full_bar[kPairStages], empty_bar[kPairStages], accf_bar[2], acce_bar[2];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int abort_flag;
   int *status = &g_linear_status;
@@ -287,8 +287,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < kPairStages; ++s) {
-      mbar_init(&full_bar[s], 1);   // this CTA's operands have landed
-      mbar_init(&peer_bar[s], 1);   // (leader) the peer's have
+      mbar_init(&full_bar[s], 1);   // (leader) both CTAs' operands have landed
       mbar_init(&empty_bar[s], 1);  // the leader's MMAs have read the stage
     }
     for (int b = 0; b < 2; ++b) {
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t m0 = int64_t(t / n_tiles) * kPairN;
       const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
       const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
-      if (!__all_sync(0xffffffffu, mbar_wait_cluster(&accf_bar[ab], (ti >> 1) & 1, &abort_flag, status, 4))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&accf_bar[ab], (ti >> 1) & 1, &abort_flag, status, 4))) break;
       tc_fence_after();
 #pragma unroll 1
       for (int c = col0; c < col0 + kPairN / 2; c += 32) {
@@ -341,26 +340,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int n0 = t % n_tiles * 2 * kBP + rank * kBP, m0 = t / n_tiles * kPairN + rank * (kPairN / 2);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
           const int s = it % kPairStages;
-          ok = mbar_wait_cluster(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, &abort_flag, status, 2);
+          ok = mbar_wait(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, &abort_flag, status, 2);
           if (!ok) break;
           uint8_t *st = smem + s * kPairStage;
-          mbar_arrive_expect_tx(&full_bar[s], kPairStage);
-          tma_load_2d(st, &wmap, kb * kBK, n0, &full_bar[s]);
-          tma_load_2d(st + kPBytes, &amap, kb * kBK, m0, &full_bar[s]);
+          const uint32_t bar = map_rank(&full_bar[s], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kPairStage);
+          tma_load_2d_pair(st, &wmap, kb * kBK, n0, bar);
+          tma_load_2d_pair(st + kPBytes, &amap, kb * kBK, m0, bar);
         }
       }
-      drain_loads(full_bar, kPairStages, it);
+      if (rank == 0) drain_loads(full_bar, kPairStages, it);
     }
-  } else if (lane == 0 && rank == 1) {
-    const uint32_t total = uint32_t(my_tiles) * uint32_t(num_kb);
-    for (uint32_t it = 0; it < total; ++it) {
-      const int s = it % kPairStages;
-      if (!mbar_wait(&full_bar[s], (it / kPairStages) & 1, &abort_flag, status, 5)) break;
-      mbar_arrive_rank(&peer_bar[s], 0);
-    }
-    // The leader's last MMAs end before this CTA frees its half of TMEM: the
-    // cluster barrier below, which the leader reaches after its last commit.
-  } else if (lane == 0) {
+  } else if (lane == 0 && rank == 0) {
     constexpr uint32_t idesc =
         (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairN >> 3) << 17) | (uint32_t(2 * kBP >> 4) << 24);
     uint32_t it = 0;
@@ -374,7 +365,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int kb = 0; kb < num_kb; ++kb, ++it) {
         const int s = it % kPairStages;
         const uint32_t ph = (it / kPairStages) & 1;
-        ok = mbar_wait(&full_bar[s], ph, &abort_flag, status, 3) && mbar_wait_cluster(&peer_bar[s], ph, &abort_flag, status, 3);
+        ok = mbar_wait(&full_bar[s], ph, &abort_flag, status, 3);
         if (!ok) break;
         tc_fence_after();
         const uint64_t da = smem_desc(smem + s * kPairStage), db = smem_desc(smem + s * kPairStage + kPBytes);
@@ -389,7 +380,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     if (done > 0) {  // every issued MMA has finished before TMEM is freed
       const long long t0 = clock64();
-      while (!mbar_try_wait_cluster(&accf_bar[(done - 1) & 1], ((done - 1) >> 1) & 1) && clock64() - t0 < kWaitCycles) {
+      while (!mbar_try_wait(&accf_bar[(done - 1) & 1], ((done - 1) >> 1) & 1) && clock64() - t0 < kWaitCycles) {
       }
     }
   }
