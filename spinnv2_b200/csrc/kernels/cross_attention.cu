@@ -13,30 +13,13 @@
 // scale * log2(e) as the factor.  A key that does not count has score -inf and
 // is read as zeros, so that what lies there (NaN included) has no influence;
 // a row without keys keeps l = 0 and is written as 0.
-#include "transformer.cuh"
+#include "cross_attention.cuh"
 
 namespace spkv2 {
 
 namespace {
 
 using namespace xf;
-
-struct AttnArgs {
-  const void *q, *k, *v;
-  void *out;
-  const int32_t *lengths;
-  const uint8_t *key_mask;
-  int64_t qs[3], ks[3], vs[3], os[3];  // batch, token, head
-  int64_t mask_stride;
-  int batch, queries, keys, kv_heads, group, width;
-  int rows;        // queries * group
-  int row_tiles;   // per (batch, key head)
-  float scale_log2;
-};
-
-__device__ __forceinline__ int entry_keys(const AttnArgs &p, int b) {
-  return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
-}
 
 // ------------------------------------------------------------ CUDA cores
 // Any type, width and alignment, exact fp32 products.  64 rows x 64 keys a
@@ -222,6 +205,7 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   a.rows = a.queries * group;
   a.scale_log2 = x->scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cross_tc_serves(a, x->dtype) && a.rows > 16) return cross_tc(a, x->dtype, s);
   return by_type(x->dtype, [&](auto t) {
     using T = decltype(t);
     if (a.width <= 32) return launch_simt<T, 32>(a, s);

@@ -1,0 +1,401 @@
+// Cross attention on the tensor cores (tcgen05, 16-bit types): many rows.
+//
+// A CTA owns 256 rows (two tiles of 128) of one entry and key head and passes
+// over the keys in tiles of 128:
+//   S = Q K^T   128 x 128 fp32 in TMEM, Q and K from shared memory (K-major)
+//   P = exp2(S * scale * log2(e) - m), rounded to the inputs' type, written
+//       back over S's columns in TMEM
+//   O += P V    A = P from TMEM, V from shared memory as it lies in memory
+//               (N-major)
+// The two tiles alternate: while the softmax warps of one work, the tensor
+// core runs the other's P V and its next Q K^T.  m is a row's running maximum,
+// lagging: O and the sum l are rescaled only when the true maximum has risen
+// by more than 2^8 over m, which bounds P by 256 and makes the rescaling (a
+// TMEM round trip of the whole O tile) rare.  The result does not depend on m.
+//
+// Warps 0-3 and 4-7: the softmax of tile 0 and 1, a row per thread; warp 8: TMA
+// of K and V; warp 9: MMA.  P is rounded once, as both operands of an MMA have
+// one type; the sums stay in fp32.
+#include "cross_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace spkv2 {
+
+namespace {
+
+using namespace xf;
+using namespace tc;
+
+constexpr int kTile = 128;  // rows of a tile, keys of a step
+constexpr int kThreads = 320;
+constexpr int kHalf = kTile * 128;  // bytes of 64 columns of a tile
+
+template <int D>
+struct Shape {
+  static constexpr int halves = D / 64;
+  static constexpr int tile_bytes = halves * kHalf;
+  static constexpr int slots = D == 128 ? 4 : 6;  // ring of K and V tiles
+  static constexpr size_t smem = size_t(2 + slots) * tile_bytes + 1024;
+};
+
+__device__ int g_cross_status;  // role code of the last bounded wait that gave up
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Which of the 128 keys from j0 on count, as four words; all lanes of a warp
+// get the same.
+__device__ __forceinline__ void key_bits(const AttnArgs &a, int b, int keys, int j0, int lane, uint32_t (&bits)[4]) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int j = j0 + w * 32 + lane;
+    bool in = j < keys;
+    if (in && a.key_mask) in = a.key_mask[b * a.mask_stride + j] != 0;
+    bits[w] = __ballot_sync(0xffffffffu, in);
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a,
+                    int k_heads_step, int k_batch_step, int v_heads_step, int v_batch_step) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using S = Shape<D>;
+  uint8_t *ring = smem + 2 * S::tile_bytes;
+  __shared__ uint64_t full_bar[S::slots], empty_bar[S::slots], q_bar, s_bar[2], p_bar[2], o_bar[2], done_bar;
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int abort_flag;
+  int *status = &g_cross_status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int t = blockIdx.x;
+  const int r0 = t % a.row_tiles * (2 * kTile);
+  t /= a.row_tiles;
+  const int hk = t % a.kv_heads, b = t / a.kv_heads;
+  const int tiles = a.rows - r0 > kTile ? 2 : 1;  // row tiles of this CTA
+
+  if (tid == 0) {
+    for (int s = 0; s < S::slots; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&q_bar, 8);
+    mbar_init(&done_bar, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_bar[i], 1);
+      mbar_init(&p_bar[i], 4);
+      mbar_init(&o_bar[i], 1);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int keys = entry_keys(a, b);
+  const int steps = (keys + kTile - 1) / kTile;
+  // TMEM columns: scores (and P) of tile i at 128 i, sums of tile i behind them.
+  auto s_col = [&](int i) { return tmem + uint32_t(i * kTile); };
+  auto o_col = [&](int i) { return tmem + uint32_t(2 * kTile + i * D); };
+
+  if (warp < 8) {
+    // ---------------------------------------------------------- softmax
+    const int i = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    {  // this warp's 32 rows of Q, swizzled for the MMA; 16-byte chunks
+      const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
+      constexpr int CH = D / 8, RPI = 32 / CH;  // chunks of a row, rows of an iteration
+      const int c = lane % CH;
+#pragma unroll 4
+      for (int k = 0; k < 32 / RPI; ++k) {
+        const int rr = quarter * 32 + k * RPI + lane / CH, row = r0 + i * kTile + rr;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < a.rows && c * 8 < a.width) {
+          const int qi = row / a.group, h = hk * a.group + row % a.group;
+          v = __ldg(reinterpret_cast<const uint4 *>(q + qi * a.qs[1] + h * a.qs[2] + c * 8));
+        }
+        *reinterpret_cast<uint4 *>(smem + i * S::tile_bytes + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_bar);
+    }
+    const int row = r0 + i * kTile + quarter * 32 + lane;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = i < tiles;
+    for (int j = 0; j < steps && ok; ++j) {
+      const bool masked = a.key_mask || (j + 1) * kTile > keys;
+      uint32_t bits[4];
+      if (masked) key_bits(a, b, keys, j * kTile, lane, bits);
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_bar[i], j & 1, &abort_flag, status, 4));
+      if (!ok) break;
+      tc_fence_after();
+      float s[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(s_col(i) + lanes + uint32_t(c), v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s[c + k] = __uint_as_float(v[k]);
+      }
+      if (masked && (bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
+#pragma unroll
+        for (int k = 0; k < kTile; ++k) s[k] = (bits[k >> 5] >> (k & 31)) & 1 ? s[k] : -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int k = 4; k < kTile; ++k) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      const bool rise = top > m + 8.0f;  // from m = -inf: any score
+      if (__any_sync(0xffffffffu, rise)) {
+        const float shrink = rise ? ex2(m - top) : 1.0f;  // 0 from m = -inf
+        if (rise) m = top;
+        l *= shrink;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(o_col(i) + lanes + uint32_t(c), v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * shrink);
+            tmem_st32(o_col(i) + lanes + uint32_t(c), v);
+          }
+        }
+      }
+      const float use = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {};
+#pragma unroll
+      for (int c = 0; c < kTile; c += 64) {
+        uint32_t p[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float e0 = ex2(fmaf(s[c + 2 * k], a.scale_log2, -use)), e1 = ex2(fmaf(s[c + 2 * k + 1], a.scale_log2, -use));
+          sum[k & 3] += e0 + e1;
+          p[k] = pack2<T>(e0, e1);
+        }
+        tmem_st32(s_col(i) + lanes + uint32_t(c / 2), p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_bar[i]);
+    }
+    // ---------------------------------------------------------- result
+    if (i < tiles && ok) {
+      if (steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_bar[i], 0, &abort_flag, status, 4));
+      tc_fence_after();
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      const int qi = row / a.group, h = hk * a.group + row % a.group;
+      T *out = static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32] = {};
+          if (steps > 0) tmem_ld32(o_col(i) + lanes + uint32_t(c), v);
+          if (row >= a.rows) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            if (c + k >= a.width) break;
+            uint4 w;
+            w.x = pack2<T>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
+            w.y = pack2<T>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+            w.z = pack2<T>(__uint_as_float(v[k + 4]) * inv, __uint_as_float(v[k + 5]) * inv);
+            w.w = pack2<T>(__uint_as_float(v[k + 6]) * inv, __uint_as_float(v[k + 7]) * inv);
+            *reinterpret_cast<uint4 *>(out + c + k) = w;
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------- K and V tiles
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int j = 0; j < steps && ok; ++j) {
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int slot = it % S::slots;
+          ok = mbar_wait(&empty_bar[slot], ((it / S::slots) & 1) ^ 1, &abort_flag, status, 2);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full_bar[slot], S::tile_bytes);
+          for (int h = 0; h < S::halves; ++h)
+            tma_load_4d(ring + slot * S::tile_bytes + h * kHalf, kv ? &vmap : &kmap, h * 64, j * kTile,
+                        hk * (kv ? v_heads_step : k_heads_step), b * (kv ? v_batch_step : k_batch_step), &full_bar[slot]);
+        }
+      }
+      // What was issued has landed before shared memory goes away.
+      for (int k = it > S::slots ? it - S::slots : 0; k < it; ++k) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full_bar[k % S::slots], (k / S::slots) & 1) && clock64() - t0 < kWaitCycles) {
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- MMA
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kTile >> 3) << 17) | (uint32_t(kTile >> 4) << 24);
+    constexpr uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kTile >> 4) << 24);
+    auto landed = [&](int it) {
+      return __all_sync(0xffffffffu, mbar_wait(&full_bar[it % S::slots], (it / S::slots) & 1, &abort_flag, status, 3));
+    };
+    auto scores = [&](int i, int slot) {  // S_i = Q_i K^T
+      const uint64_t dq = smem_desc(smem + i * S::tile_bytes), dk = smem_desc(ring + slot * S::tile_bytes);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint64_t off = uint64_t((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+        mma_f16(s_col(i), dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
+      }
+    };
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&q_bar, 0, &abort_flag, status, 3));
+    if (ok && steps > 0) {
+      ok = landed(0);
+      if (ok && lane == 0) {
+        tc_fence_after();
+        for (int i = 0; i < tiles; ++i) {
+          scores(i, 0);
+          mma_commit(&s_bar[i]);
+        }
+        mma_commit(&empty_bar[0]);
+      }
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      const int vs = (2 * j + 1) % S::slots, kn = (2 * j + 2) % S::slots;
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      if (a.key_mask || (j + 1) * kTile > keys) key_bits(a, b, keys, j * kTile, lane, bits);
+      ok = landed(2 * j + 1);
+      if (!ok) break;
+      if ((bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
+        // Values that do not count meet p = 0 in the MMA: they must be finite.
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          for (uint32_t off = ~bits[w]; off; off &= off - 1)
+            if (lane < S::halves * 8)
+              *reinterpret_cast<uint4 *>(ring + vs * S::tile_bytes + (lane >> 3) * kHalf + (w * 32 + __ffs(off) - 1) * 128 +
+                                         (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+      }
+      for (int i = 0; i < tiles && ok; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&p_bar[i], j & 1, &abort_flag, status, 7));
+        if (!ok) break;
+        if (i == 0 && j + 1 < steps) {
+          ok = landed(2 * j + 2);
+          if (!ok) break;
+        }
+        if (lane == 0) {
+          tc_fence_after();
+          const uint64_t dv = smem_desc_mn(ring + vs * S::tile_bytes, kHalf);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+            mma_f16_ta(o_col(i), s_col(i) + uint32_t(k * 8), dv + (uint64_t(k * 16 * 128) >> 4), id_o, (j | k) ? 1u : 0u);
+          if (i == tiles - 1) mma_commit(&empty_bar[vs]);
+          if (j + 1 < steps) {
+            scores(i, kn);
+            mma_commit(&s_bar[i]);
+            if (i == tiles - 1) mma_commit(&empty_bar[kn]);
+          } else {
+            mma_commit(&o_bar[i]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) {  // every issued MMA has finished before TMEM is freed, also after a wait that gave up
+      mma_commit(&done_bar);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&done_bar, 0) && clock64() - t0 < kWaitCycles) {
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+struct Map {
+  CUtensorMap map;
+  int heads_step, batch_step;  // 0: one head or entry for all (stride 0)
+};
+
+bool encode_kv(Map *m, const AttnArgs &a, const void *base, const int64_t (&st)[3]) {
+  m->heads_step = st[2] != 0 && a.kv_heads > 1;
+  m->batch_step = st[0] != 0 && a.batch > 1;
+  const cuuint64_t dims[4] = {cuuint64_t(a.width), cuuint64_t(a.keys), cuuint64_t(m->heads_step ? a.kv_heads : 1),
+                              cuuint64_t(m->batch_step ? a.batch : 1)};
+  const cuuint64_t any = (cuuint64_t(a.width) * 2 + 15) / 16 * 16;
+  const cuuint64_t strides[3] = {a.keys > 1 ? cuuint64_t(st[1]) * 2 : any, m->heads_step ? cuuint64_t(st[2]) * 2 : any,
+                                 m->batch_step ? cuuint64_t(st[0]) * 2 : any};
+  const cuuint32_t box[4] = {64, kTile, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode_fn()(&m->map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D>
+int launch(AttnArgs a, cudaStream_t s) {
+  a.row_tiles = int(ceil_div(a.rows, 2 * kTile));
+  const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
+  if (blocks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  if (const int rc = allow_smem<cross_tc_kernel<T, D>>(Shape<D>::smem)) return rc;
+  Map k, v;
+  if (!encode_kv(&k, a, a.k, a.ks) || !encode_kv(&v, a, a.v, a.vs)) return SPKV2_ERR_CUDA;
+  return cuda_status(launch_kernel(cross_tc_kernel<T, D>, unsigned(blocks), kThreads, Shape<D>::smem, s, 1, k.map, v.map, a,
+                                   k.heads_step, k.batch_step, v.heads_step, v.batch_step));
+}
+
+bool rows_aligned(const void *base, const int64_t (&st)[3]) {
+  return aligned16(base) && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0;
+}
+
+// Strides that a tensor map can hold.
+bool mappable(const AttnArgs &a, const int64_t (&st)[3]) {
+  const int64_t most = int64_t(1) << 38;
+  return (a.keys == 1 || st[1] > 0) && st[0] < most && st[1] < most && st[2] < most;
+}
+
+}  // namespace
+
+bool cross_tc_serves(const AttnArgs &a, int32_t dtype) {
+  return elem_bytes(dtype) == 2 && a.width <= 128 && a.width % 8 == 0 && a.keys > 0 && a.scale_log2 > 0.0f && encode_fn() &&
+         rows_aligned(a.q, a.qs) && rows_aligned(a.k, a.ks) && rows_aligned(a.v, a.vs) && rows_aligned(a.out, a.os) &&
+         mappable(a, a.ks) && mappable(a, a.vs);
+}
+
+int cross_tc(const AttnArgs &a, int32_t dtype, cudaStream_t s) {
+  if (dtype == SPKV2_DTYPE_FP16) return a.width <= 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+  return a.width <= 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace spkv2
