@@ -205,7 +205,7 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   a.rows = a.queries * group;
   a.scale_log2 = x->scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cross_tc_serves(a, x->dtype) && a.rows > 16) return cross_tc(a, x->dtype, s);
+  if (cross_tc_serves(a, x->dtype)) return a.rows <= 32 ? cross_step(a, x->dtype, s) : cross_tc(a, x->dtype, s);
   return by_type(x->dtype, [&](auto t) {
     using T = decltype(t);
     if (a.width <= 32) return launch_simt<T, 32>(a, s);

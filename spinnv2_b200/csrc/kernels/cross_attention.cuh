@@ -1,8 +1,10 @@
 // Arguments shared by the cross attention kernels: cross_attention.cu (CUDA
-// cores, any type and alignment, and the choice between the kernels) and
-// cross_attention_tc.cu (tcgen05, 16-bit types, many rows).
+// cores, any type and alignment, and the choice between the kernels),
+// cross_attention_tc.cu (tcgen05, 16-bit types, many rows) and
+// cross_attention_step.cu (mma.sync, 16-bit types, few rows).
 #pragma once
 
+#include "tcgen05.cuh"
 #include "transformer.cuh"
 
 namespace spkv2 {
@@ -24,9 +26,32 @@ __device__ __forceinline__ int entry_keys(const AttnArgs &p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
 }
 
-// Whether the tensor-core kernel takes these arguments: 16-bit elements, width
+// Tensor map of keys or values as {width, key, head, entry}, 128-byte swizzle,
+// boxes of 64 columns x `box_keys` keys.
+struct KvMap {
+  CUtensorMap map;
+  int heads_step, batch_step;  // 0: one head or entry for all (stride 0)
+};
+
+inline bool encode_kv(KvMap *m, const AttnArgs &a, const void *base, const int64_t (&st)[3], int box_keys) {
+  m->heads_step = st[2] != 0 && a.kv_heads > 1;
+  m->batch_step = st[0] != 0 && a.batch > 1;
+  const cuuint64_t dims[4] = {cuuint64_t(a.width), cuuint64_t(a.keys), cuuint64_t(m->heads_step ? a.kv_heads : 1),
+                              cuuint64_t(m->batch_step ? a.batch : 1)};
+  const cuuint64_t any = (cuuint64_t(a.width) * 2 + 15) / 16 * 16;
+  const cuuint64_t strides[3] = {a.keys > 1 ? cuuint64_t(st[1]) * 2 : any, m->heads_step ? cuuint64_t(st[2]) * 2 : any,
+                                 m->batch_step ? cuuint64_t(st[0]) * 2 : any};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_keys), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return tc::encode_fn()(&m->map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether the tensor-core kernels take these arguments: 16-bit elements, width
 // a multiple of 8 up to 128, rows on 16-byte boundaries, a positive scale.
 bool cross_tc_serves(const AttnArgs &a, int32_t dtype);
 int cross_tc(const AttnArgs &a, int32_t dtype, cudaStream_t s);
+int cross_step(const AttnArgs &a, int32_t dtype, cudaStream_t s);  // a.rows <= 32
 
 }  // namespace spkv2

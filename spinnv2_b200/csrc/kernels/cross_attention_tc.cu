@@ -343,34 +343,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-struct Map {
-  CUtensorMap map;
-  int heads_step, batch_step;  // 0: one head or entry for all (stride 0)
-};
-
-bool encode_kv(Map *m, const AttnArgs &a, const void *base, const int64_t (&st)[3]) {
-  m->heads_step = st[2] != 0 && a.kv_heads > 1;
-  m->batch_step = st[0] != 0 && a.batch > 1;
-  const cuuint64_t dims[4] = {cuuint64_t(a.width), cuuint64_t(a.keys), cuuint64_t(m->heads_step ? a.kv_heads : 1),
-                              cuuint64_t(m->batch_step ? a.batch : 1)};
-  const cuuint64_t any = (cuuint64_t(a.width) * 2 + 15) / 16 * 16;
-  const cuuint64_t strides[3] = {a.keys > 1 ? cuuint64_t(st[1]) * 2 : any, m->heads_step ? cuuint64_t(st[2]) * 2 : any,
-                                 m->batch_step ? cuuint64_t(st[0]) * 2 : any};
-  const cuuint32_t box[4] = {64, kTile, 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return encode_fn()(&m->map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <class T, int D>
 int launch(AttnArgs a, cudaStream_t s) {
   a.row_tiles = int(ceil_div(a.rows, 2 * kTile));
   const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
   if (blocks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
   if (const int rc = allow_smem<cross_tc_kernel<T, D>>(Shape<D>::smem)) return rc;
-  Map k, v;
-  if (!encode_kv(&k, a, a.k, a.ks) || !encode_kv(&v, a, a.v, a.vs)) return SPKV2_ERR_CUDA;
+  KvMap k, v;
+  if (!encode_kv(&k, a, a.k, a.ks, kTile) || !encode_kv(&v, a, a.v, a.vs, kTile)) return SPKV2_ERR_CUDA;
   return cuda_status(launch_kernel(cross_tc_kernel<T, D>, unsigned(blocks), kThreads, Shape<D>::smem, s, 1, k.map, v.map, a,
                                    k.heads_step, k.batch_step, v.heads_step, v.batch_step));
 }
