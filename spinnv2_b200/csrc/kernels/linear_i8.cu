@@ -121,12 +121,65 @@ __device__ __forceinline__ void store_chunk(const LinearArgs &p, const uint32_t 
     if (j < cnt) y[j * p.y_stride] = from_f32<T>(v[j]);
 }
 
+constexpr int kSplitThreads = 192;
+
+// Columns c0 .. c1 - 1 of the cluster's partial sums part[column][channel], added
+// up and stored: a warp per column, four channels a lane, four columns' loads
+// from every CTA in flight.
+template <class T>
+__device__ __forceinline__ void join_columns(const LinearArgs &p, const int32_t *part, int64_t n0, int64_t m0, int c0, int c1,
+                                             int csize, int warp, int lane) {
+  constexpr int WARPS = kSplitThreads / 32, U = 4;
+  const int64_t n = n0 + lane * 4;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    sw[e] = n + e < p.n ? __ldg(p.w_scale + n + e) : 0.0f;
+    bias[e] = p.bias && n + e < p.n ? __ldg(p.bias + n + e) : 0.0f;
+  }
+  const int end = int(min(int64_t(c1), p.m - m0));  // columns past m are padding
+  const bool vec = n + 4 <= p.n && p.y_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
+  for (int c = c0 + warp; c < end; c += WARPS * U) {
+    int4 sum[U] = {};
+    float sa[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sa[u] = c + u * WARPS < end ? __ldg(p.a_scale + m0 + c + u * WARPS) : 0.0f;
+#pragma unroll 2
+    for (int r = 0; r < csize; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u * WARPS < end) {
+          const int4 v = ld_cluster4(map_rank(part + (c + u * WARPS) * kBP + lane * 4, uint32_t(r)));
+          sum[u].x += v.x, sum[u].y += v.y, sum[u].z += v.z, sum[u].w += v.w;
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u * WARPS >= end) break;
+      const float v[4] = {linear_value(sum[u].x, sa[u], sw[0], bias[0], p.act), linear_value(sum[u].y, sa[u], sw[1], bias[1], p.act),
+                          linear_value(sum[u].z, sa[u], sw[2], bias[2], p.act), linear_value(sum[u].w, sa[u], sw[3], bias[3], p.act)};
+      T *y = static_cast<T *>(p.y) + (m0 + c + u * WARPS) * p.y_stride + n;
+      if (vec) {
+        struct alignas(4 * sizeof(T)) Four {
+          T v[4];
+        };
+        Four f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[e] = from_f32<T>(v[e]);
+        *reinterpret_cast<Four *>(y) = f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.n) y[e] = from_f32<T>(v[e]);
+      }
+    }
+  }
+}
+
 // Few tiles: one tile of 128 channels x BN tokens per cluster, whose CTAs
 // divide k.  Each CTA leaves its int32 sums in its own shared memory and
 // takes BN / cluster columns of everybody's: integer sums, so the order does
 // not matter, and nothing passes through global memory.  Warps 0-3 epilogue,
 // 4 TMA producer, 5 MMA.
-constexpr int kSplitThreads = 192;
 constexpr int split_stages(int bn) { return bn >= 256 ? 4 : bn == 128 ? 6 : bn == 64 ? 8 : 10; }
 constexpr size_t split_smem(int bn) { return size_t(split_stages(bn)) * (kPBytes + bn * kBK) + 1024; }
 
@@ -199,7 +252,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       }
     }
   } else if (warp == 4) {
-    if (lane == 0) {
+    if (elect_one()) {
       int it = 0;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % STAGES;
@@ -211,7 +264,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       }
       drain_loads(full_bar, STAGES, uint32_t(it));
     }
-  } else if (lane == 0) {
+  } else if (elect_one()) {
     constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBP >> 4) << 24);
     for (int kb = kb0; kb < kb1; ++kb) {
       const int it = kb - kb0, s = it % STAGES;
@@ -228,21 +281,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncwarp();
   if (csize > 1) {
     cluster_sync();
-    if (warp < 4 && !abort_flag) {
-      const int per = BN / csize;
-      const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
-      const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
-#pragma unroll 1
-      for (int c = rank * per; c < (rank + 1) * per; ++c) {
-        const int64_t m = m0 + c;
-        if (m >= p.m) break;
-        const int32_t *own = part + c * kBP + warp * 32 + lane;
-        int sum = 0;
-        for (int r = 0; r < csize; ++r) sum += int(ld_cluster(map_rank(own, uint32_t(r))));
-        if (n < p.n)
-          static_cast<T *>(p.y)[m * p.y_stride + n] = from_f32<T>(linear_value(sum, __ldg(p.a_scale + m), sw, bias, p.act));
-      }
-    }
+    if (!abort_flag) join_columns<T>(p, part, n0, m0, rank * (BN / csize), (rank + 1) * (BN / csize), csize, warp, lane);
     __syncwarp();
     cluster_sync();  // the peers have read this CTA's sums
   }
@@ -332,7 +371,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else if (warp == 8) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
       for (int ti = 0; ti < my_tiles && ok; ++ti) {
@@ -351,7 +390,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       if (rank == 0) drain_loads(full_bar, kPairStages, it);
     }
-  } else if (lane == 0 && rank == 0) {
+  } else if (rank == 0 && elect_one()) {
     constexpr uint32_t idesc =
         (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairN >> 3) << 17) | (uint32_t(2 * kBP >> 4) << 24);
     uint32_t it = 0;

@@ -325,6 +325,12 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // All threads of both CTAs: barrier across the cluster.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
