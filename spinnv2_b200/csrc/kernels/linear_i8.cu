@@ -21,6 +21,7 @@ struct LinearArgs {
   void *y;
   int64_t m, n, a_stride, w_stride, y_stride;
   int k, act;
+  int y_tma;  // y can be stored by TMA
 };
 
 __device__ __forceinline__ float linear_value(int acc, float sa, float sw, float bias, int act) {
@@ -103,18 +104,71 @@ __device__ __forceinline__ void drain_loads(uint64_t *full_bar, int stages, uint
   }
 }
 
-// A chunk of COLS (at most 32) accumulator columns: tokens m, m + 1, .. of this
-// thread's channel.
+// Four channels n .. n + 3 of one token, scaled and stored; `vec`: all four
+// exist and their place is aligned for one store.
+template <class T>
+__device__ __forceinline__ void store4(const LinearArgs &p, const int4 acc, int64_t m, int64_t n, float sa, const float (&sw)[4],
+                                       const float (&bias)[4], bool vec, bool real) {
+  float v[4] = {fmaf(float(acc.x) * sa, sw[0], bias[0]), fmaf(float(acc.y) * sa, sw[1], bias[1]),
+                fmaf(float(acc.z) * sa, sw[2], bias[2]), fmaf(float(acc.w) * sa, sw[3], bias[3])};
+  apply_act_n<4>(v, p.act);
+  T *y = static_cast<T *>(p.y) + m * p.y_stride + n;
+  if (vec) {
+    struct alignas(4 * sizeof(T)) Four {
+      T v[4];
+    };
+    Four f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.v[e] = from_f32<T>(v[e]);
+    if (real) *reinterpret_cast<Four *>(y) = f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (real && n + e < p.n) y[e] = from_f32<T>(v[e]);
+  }
+}
+template <class T>
+__device__ __forceinline__ bool vec4_out(const LinearArgs &p, int64_t n) {
+  return n + 4 <= p.n && p.y_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
+}
+__device__ __forceinline__ void load_channels(const LinearArgs &p, int64_t n, float (&sw)[4], float (&bias)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    sw[e] = n + e < p.n ? __ldg(p.w_scale + n + e) : 0.0f;
+    bias[e] = p.bias && n + e < p.n ? __ldg(p.bias + n + e) : 0.0f;
+  }
+}
+
+// A warp's chunk of accumulators: COLS tokens from m on of channel n (a lane
+// each; n0 the warp's first).  Where rows of y lie on 16-byte boundaries the
+// chunk goes through one of the warp's two buffers of 32 tokens x 32 channels
+// and one TMA store, which takes the stores off the warps: 32 two-byte stores a
+// lane made the epilogue longer than a tile's MMAs (12544 x 256 x 2048 in bf16:
+// 33 us, with TMA stores 27 us).  `count`: the chunks this warp has stored.
 template <class T, int COLS>
-__device__ __forceinline__ void store_chunk(const LinearArgs &p, const uint32_t (&acc)[32], int64_t n, int64_t m, int lane,
-                                            float sw, float bias) {
+__device__ __forceinline__ void store_chunk(const LinearArgs &p, const CUtensorMap *ymap, T *buffers, int &count,
+                                            const uint32_t (&acc)[32], int64_t n0, int64_t m, int lane, float sw, float bias) {
+  const int64_t n = n0 + lane;
   const float mine = m + lane < p.m ? __ldg(p.a_scale + m + lane) : 0.0f;
-  const int cnt = int(min(int64_t(COLS), p.m - m));
   float v[32];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = fmaf(float(int(acc[j])) * __shfl_sync(0xffffffffu, mine, j), sw, bias);
-  apply_act32(v, p.act);
+  for (int j = 0; j < COLS; ++j) v[j] = fmaf(float(int(acc[j])) * __shfl_sync(0xffffffffu, mine, j), sw, bias);
+  if (p.act != SPKV2_CUDA_ACT_NONE) apply_act32(v, p.act);
+  if (COLS == 32 && p.y_tma) {
+    if (n0 >= p.n) return;
+    T *buf = buffers + (count & 1) * 1024;
+    if (lane == 0) tma_store_wait_read1();  // the store before the last has read this buffer
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) buf[j * 32 + lane] = from_f32<T>(v[j]);
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) tma_store_2d(ymap, int(n0), int(m), buf);
+    ++count;
+    return;
+  }
   if (n >= p.n) return;
+  const int cnt = int(min(int64_t(COLS), p.m - m));
   T *y = static_cast<T *>(p.y) + m * p.y_stride + n;
 #pragma unroll
   for (int j = 0; j < COLS; ++j)
@@ -132,13 +186,9 @@ __device__ __forceinline__ void join_columns(const LinearArgs &p, const int32_t 
   constexpr int WARPS = kSplitThreads / 32, U = 4;
   const int64_t n = n0 + lane * 4;
   float sw[4], bias[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    sw[e] = n + e < p.n ? __ldg(p.w_scale + n + e) : 0.0f;
-    bias[e] = p.bias && n + e < p.n ? __ldg(p.bias + n + e) : 0.0f;
-  }
+  load_channels(p, n, sw, bias);
   const int end = int(min(int64_t(c1), p.m - m0));  // columns past m are padding
-  const bool vec = n + 4 <= p.n && p.y_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
+  const bool vec = vec4_out<T>(p, n);
   for (int c = c0 + warp; c < end; c += WARPS * U) {
     int4 sum[U] = {};
     float sa[U];
@@ -153,25 +203,8 @@ __device__ __forceinline__ void join_columns(const LinearArgs &p, const int32_t 
           sum[u].x += v.x, sum[u].y += v.y, sum[u].z += v.z, sum[u].w += v.w;
         }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + u * WARPS >= end) break;
-      const float v[4] = {linear_value(sum[u].x, sa[u], sw[0], bias[0], p.act), linear_value(sum[u].y, sa[u], sw[1], bias[1], p.act),
-                          linear_value(sum[u].z, sa[u], sw[2], bias[2], p.act), linear_value(sum[u].w, sa[u], sw[3], bias[3], p.act)};
-      T *y = static_cast<T *>(p.y) + (m0 + c + u * WARPS) * p.y_stride + n;
-      if (vec) {
-        struct alignas(4 * sizeof(T)) Four {
-          T v[4];
-        };
-        Four f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.v[e] = from_f32<T>(v[e]);
-        *reinterpret_cast<Four *>(y) = f;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.n) y[e] = from_f32<T>(v[e]);
-      }
-    }
+    for (int u = 0; u < U; ++u)
+      store4<T>(p, sum[u], m0 + c + u * WARPS, n, sa[u], sw, bias, vec, c + u * WARPS < end);
   }
 }
 
@@ -185,8 +218,8 @@ constexpr size_t split_smem(int bn) { return size_t(split_stages(bn)) * (kPBytes
 
 template <class T, int BN>
 __global__ void __launch_bounds__(kSplitThreads, 1)
-    linear_split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap, LinearArgs p,
-                        int n_tiles, int num_kb, int csize) {
+    linear_split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap,
+                        const __grid_constant__ CUtensorMap ymap, LinearArgs p, int n_tiles, int num_kb, int csize) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int STAGES = split_stages(BN);
@@ -225,22 +258,25 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   pdl_wait();
 
   const uint32_t trow = tmem + (uint32_t(warp * 32) << 16);
-  const int64_t n = n0 + warp * 32 + lane;  // warps 0-3
   int32_t *part = reinterpret_cast<int32_t *>(smem);  // [column][channel]
   bool landed = false;
   if (warp < 4) {
     landed = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0, &abort_flag, status, 4));
     tc_fence_after();
     if (landed && csize == 1) {
+      const int64_t n = n0 + warp * 32 + lane;
       const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
       const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+      int count = 0;
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
         if (m0 + c >= p.m) break;
         uint32_t acc[32];
         tmem_ld32(trow + uint32_t(c), acc);
-        store_chunk<T, BN < 32 ? BN : 32>(p, acc, n, m0 + c, lane, sw, bias);
+        store_chunk<T, BN < 32 ? BN : 32>(p, &ymap, reinterpret_cast<T *>(part) + warp * 2048, count, acc, n0 + warp * 32, m0 + c,
+                                          lane, sw, bias);
       }
+      if (lane == 0) tma_store_wait_all();
     } else if (landed) {
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
@@ -305,17 +341,19 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // more than L2 can give every SM).  Two accumulator buffers in TMEM: a tile's
 // epilogue runs under the next tile's MMAs.  Warps 0-7 epilogue, 8 TMA
 // producer, 9 MMA (in the leader).
-constexpr int kPairThreads = 320, kPairN = 256, kPairStages = 6;
+constexpr int kPairThreads = 320, kPairN = 256;
 constexpr int kPairStage = kPBytes + kPairN / 2 * kBK;
-constexpr size_t kPairSmem = size_t(kPairStages) * kPairStage + 1024;
+constexpr int pair_stages(int elem) { return elem == 4 ? 5 : 6; }
+constexpr size_t pair_smem(int elem) { return size_t(pair_stages(elem)) * kPairStage + 8 * 2048 * elem + 1024; }
 
 template <class T>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap, LinearArgs p,
-                       int n_tiles, int tiles, int num_kb) {
+    linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap,
+                       const __grid_constant__ CUtensorMap ymap, LinearArgs p, int n_tiles, int tiles, int num_kb) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full_bar[kPairStages], empty_bar[kPairStages], accf_bar[2], acce_bar[2];
+  constexpr int STAGES = pair_stages(sizeof(T));
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], accf_bar[2], acce_bar[2];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int abort_flag;
   int *status = &g_linear_status;
@@ -325,7 +363,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int my_tiles = tile0 < tiles ? (tiles - 1 - tile0) / tstep + 1 : 0;
 
   if (tid == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);   // (leader) both CTAs' operands have landed
       mbar_init(&empty_bar[s], 1);  // the leader's MMAs have read the stage
     }
@@ -350,6 +388,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   if (warp < 8) {
     const int quarter = warp & 3, col0 = (warp >> 2) * (kPairN / 2);
+    T *buffers = reinterpret_cast<T *>(smem + STAGES * kPairStage) + warp * 2048;
+    int count = 0;
     for (int ti = 0; ti < my_tiles; ++ti) {
       const int t = tile0 + ti * tstep, ab = ti & 1;
       const int64_t n = int64_t(t % n_tiles) * 2 * kBP + rank * kBP + quarter * 32 + lane;
@@ -365,11 +405,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (c + 32 == col0 + kPairN / 2) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_rank(&acce_bar[ab], 0);
+          if (lane == 0) mbar_arrive_rank_tmem(&acce_bar[ab], 0);
         }
-        if (m0 + c < p.m) store_chunk<T, 32>(p, acc, n, m0 + c, lane, sw, bias);
+        if (m0 + c < p.m) store_chunk<T, 32>(p, &ymap, buffers, count, acc, n - lane, m0 + c, lane, sw, bias);
       }
     }
+    if (lane == 0) tma_store_wait_all();
   } else if (warp == 8) {
     if (elect_one()) {
       uint32_t it = 0;
@@ -378,8 +419,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int t = tile0 + ti * tstep;
         const int n0 = t % n_tiles * 2 * kBP + rank * kBP, m0 = t / n_tiles * kPairN + rank * (kPairN / 2);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = it % kPairStages;
-          ok = mbar_wait(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, &abort_flag, status, 2);
+          const int s = it % STAGES;
+          ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, &abort_flag, status, 2);
           if (!ok) break;
           uint8_t *st = smem + s * kPairStage;
           const uint32_t bar = map_rank(&full_bar[s], 0);
@@ -388,7 +429,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tma_load_2d_pair(st + kPBytes, &amap, kb * kBK, m0, bar);
         }
       }
-      if (rank == 0) drain_loads(full_bar, kPairStages, it);
+      if (rank == 0) drain_loads(full_bar, STAGES, it);
     }
   } else if (rank == 0 && elect_one()) {
     constexpr uint32_t idesc =
@@ -402,8 +443,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!ok) break;
       tc_fence_after();
       for (int kb = 0; kb < num_kb; ++kb, ++it) {
-        const int s = it % kPairStages;
-        const uint32_t ph = (it / kPairStages) & 1;
+        const int s = it % STAGES;
+        const uint32_t ph = (it / STAGES) & 1;
         ok = mbar_wait(&full_bar[s], ph, &abort_flag, status, 3);
         if (!ok) break;
         tc_fence_after();
@@ -443,32 +484,48 @@ bool encode_rows(CUtensorMap *map, const int8_t *base, int64_t rows, int64_t str
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, uint64_t(k), uint64_t(rows), pitch, uint32_t(box));
 }
 
+// Stores of 32 channels x 32 tokens; false where rows of y are not on 16-byte
+// boundaries.
+template <class T>
+bool encode_y(CUtensorMap *map, const LinearArgs &p) {
+  if (!aligned16(p.y) || (p.m > 1 && p.y_stride * int64_t(sizeof(T)) % 16 != 0)) return false;
+  const uint64_t pitch = p.m > 1 ? uint64_t(p.y_stride) : (uint64_t(p.n) + 7) / 8 * 8;
+  return encode_2d_box(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T), p.y,
+                       uint64_t(p.n), uint64_t(p.m), pitch, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <class T, int BN>
-int launch_split(const LinearArgs &p, int n_tiles, int m_tiles, int num_kb, int csize, cudaStream_t s) {
+int launch_split(const LinearArgs &p, const CUtensorMap &ymap, int n_tiles, int m_tiles, int num_kb, int csize, cudaStream_t s) {
   if (const int rc = allow_smem<linear_split_kernel<T, BN>>(split_smem(BN))) return rc;
   CUtensorMap wmap, amap;
   if (!encode_rows(&wmap, p.w, p.n, p.w_stride, p.k, kBP) || !encode_rows(&amap, p.a, p.m, p.a_stride, p.k, BN))
     return SPKV2_ERR_CUDA;
-  return cuda_status(launch_kernel(linear_split_kernel<T, BN>, unsigned(n_tiles * m_tiles * csize), kSplitThreads, split_smem(BN), s, csize, wmap,
-                                   amap, p, n_tiles, num_kb, csize));
+  // A CTA with fewer K steps than stages asks for what it uses: less shared
+  // memory, so that clusters find room beside one another.
+  const size_t used = std::max(size_t(std::min(split_stages(BN), int(ceil_div(num_kb, csize)))) * (kPBytes + BN * kBK),
+                               size_t(csize > 1 ? BN * kBP * 4 : 4 * 2048 * int(sizeof(T)))) + 1024;
+  return cuda_status(launch_kernel(linear_split_kernel<T, BN>, unsigned(n_tiles * m_tiles * csize), kSplitThreads, used, s, csize,
+                                   wmap, amap, ymap, p, n_tiles, num_kb, csize));
 }
 
 template <class T>
-int launch_pair(const LinearArgs &p, int n_tiles, int m_tiles, int num_kb, cudaStream_t s) {
-  if (const int rc = allow_smem<linear_pair_kernel<T>>(kPairSmem)) return rc;
+int launch_pair(const LinearArgs &p, const CUtensorMap &ymap, int n_tiles, int m_tiles, int num_kb, cudaStream_t s) {
+  if (const int rc = allow_smem<linear_pair_kernel<T>>(pair_smem(sizeof(T)))) return rc;
   CUtensorMap wmap, amap;
   if (!encode_rows(&wmap, p.w, p.n, p.w_stride, p.k, kBP) || !encode_rows(&amap, p.a, p.m, p.a_stride, p.k, kPairN / 2))
     return SPKV2_ERR_CUDA;
   const int tiles = n_tiles * m_tiles;
-  return cuda_status(launch_kernel(linear_pair_kernel<T>, 2u * unsigned(std::min(tiles, sm_count() / 2)), kPairThreads, kPairSmem, s, 2, wmap,
-                                   amap, p, n_tiles, tiles, num_kb));
+  return cuda_status(launch_kernel(linear_pair_kernel<T>, 2u * unsigned(std::min(tiles, sm_count() / 2)), kPairThreads, pair_smem(sizeof(T)),
+                                   s, 2, wmap, amap, ymap, p, n_tiles, tiles, num_kb));
 }
 
 // The cheapest shape by the cycles of its busiest SM: MMA steps (2 cycles for
 // each token column of a K step) or operand bytes (64 a cycle from L2),
 // whichever is more, times the tiles it runs one after another.
 template <class T>
-int launch_tc(const LinearArgs &p, cudaStream_t s) {
+int launch_tc(LinearArgs p, cudaStream_t s) {
+  CUtensorMap ymap = {};
+  p.y_tma = encode_y<T>(&ymap, p);
   const int num_kb = int(ceil_div(p.k, kBK)), sms = sm_count();
   const int64_t n_tiles = ceil_div(p.n, kBP);
   int best_bn = 0, best_c = 1;
@@ -485,14 +542,14 @@ int launch_tc(const LinearArgs &p, cudaStream_t s) {
   }
   const int64_t pn = ceil_div(p.n, 2 * kBP), pm = ceil_div(p.m, kPairN);
   const double pair = double(ceil_div(pn * pm, sms / 2)) * num_kb * 512.0 + 4000.0;
-  if (pn * pm <= INT32_MAX / 2 && (pair < best || !best_bn)) return launch_pair<T>(p, int(pn), int(pm), num_kb, s);
+  if (pn * pm <= INT32_MAX / 2 && (pair < best || !best_bn)) return launch_pair<T>(p, ymap, int(pn), int(pm), num_kb, s);
   const int nt = int(n_tiles), mt = int(ceil_div(p.m, best_bn));
   switch (best_bn) {
-    case 16: return launch_split<T, 16>(p, nt, mt, num_kb, best_c, s);
-    case 32: return launch_split<T, 32>(p, nt, mt, num_kb, best_c, s);
-    case 64: return launch_split<T, 64>(p, nt, mt, num_kb, best_c, s);
-    case 128: return launch_split<T, 128>(p, nt, mt, num_kb, best_c, s);
-    default: return launch_split<T, 256>(p, nt, mt, num_kb, best_c, s);
+    case 16: return launch_split<T, 16>(p, ymap, nt, mt, num_kb, best_c, s);
+    case 32: return launch_split<T, 32>(p, ymap, nt, mt, num_kb, best_c, s);
+    case 64: return launch_split<T, 64>(p, ymap, nt, mt, num_kb, best_c, s);
+    case 128: return launch_split<T, 128>(p, ymap, nt, mt, num_kb, best_c, s);
+    default: return launch_split<T, 256>(p, ymap, nt, mt, num_kb, best_c, s);
   }
 }
 

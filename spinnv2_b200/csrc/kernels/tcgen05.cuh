@@ -345,6 +345,13 @@ __device__ __forceinline__ void mbar_arrive_rank(uint64_t *bar, uint32_t rank) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 
+// The same for arrivals that hand over TMEM only (tc_fence_before() precedes
+// them): no ordering of this thread's other memory accesses at cluster scope,
+// which would wait for its global stores.
+__device__ __forceinline__ void mbar_arrive_rank_tmem(uint64_t *bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_rank(bar, rank)) : "memory");
+}
+
 // Bounded probe with acquire at cluster scope (for barriers that receive
 // arrivals from the peer CTA).
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
