@@ -141,23 +141,30 @@ __device__ __forceinline__ void load_channels(const LinearArgs &p, int64_t n, fl
 
 // A warp's chunk of accumulators: COLS tokens from m on of channel n (a lane
 // each; n0 the warp's first).  Where rows of y lie on 16-byte boundaries the
-// chunk goes through one of the warp's two buffers of 32 tokens x 32 channels
+// chunk goes through one of the warp's BUFS buffers of 32 tokens x 32 channels
 // and one TMA store, which takes the stores off the warps: 32 two-byte stores a
 // lane made the epilogue longer than a tile's MMAs (12544 x 256 x 2048 in bf16:
-// 33 us, with TMA stores 27 us).  `count`: the chunks this warp has stored.
-template <class T, int COLS>
+// 31 us, with TMA stores 18.4 us).  `mine`: the
+// scale of token m + lane; `count`: the chunks this warp has stored.
+__device__ __forceinline__ float token_scale(const LinearArgs &p, int64_t m) { return m < p.m ? __ldg(p.a_scale + m) : 0.0f; }
+
+template <class T, int COLS, int BUFS>
 __device__ __forceinline__ void store_chunk(const LinearArgs &p, const CUtensorMap *ymap, T *buffers, int &count,
-                                            const uint32_t (&acc)[32], int64_t n0, int64_t m, int lane, float sw, float bias) {
+                                            const uint32_t (&acc)[32], int64_t n0, int64_t m, int lane, float mine, float sw, float bias) {
   const int64_t n = n0 + lane;
-  const float mine = m + lane < p.m ? __ldg(p.a_scale + m + lane) : 0.0f;
   float v[32];
 #pragma unroll
   for (int j = 0; j < COLS; ++j) v[j] = fmaf(float(int(acc[j])) * __shfl_sync(0xffffffffu, mine, j), sw, bias);
   if (p.act != SPKV2_CUDA_ACT_NONE) apply_act32(v, p.act);
   if (COLS == 32 && p.y_tma) {
     if (n0 >= p.n) return;
-    T *buf = buffers + (count & 1) * 1024;
-    if (lane == 0) tma_store_wait_read1();  // the store before the last has read this buffer
+    T *buf = buffers + (count & (BUFS - 1)) * 1024;
+    if (lane == 0) {  // the last store from this buffer has read it
+      if (BUFS == 2)
+        tma_store_wait_read1();
+      else
+        tma_store_wait_read0();
+    }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < COLS; ++j) buf[j * 32 + lane] = from_f32<T>(v[j]);
@@ -273,8 +280,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         if (m0 + c >= p.m) break;
         uint32_t acc[32];
         tmem_ld32(trow + uint32_t(c), acc);
-        store_chunk<T, BN < 32 ? BN : 32>(p, &ymap, reinterpret_cast<T *>(part) + warp * 2048, count, acc, n0 + warp * 32, m0 + c,
-                                          lane, sw, bias);
+        store_chunk<T, BN < 32 ? BN : 32, 2>(p, &ymap, reinterpret_cast<T *>(part) + warp * 2048, count, acc, n0 + warp * 32, m0 + c,
+                                          lane, token_scale(p, m0 + c + lane), sw, bias);
       }
       if (lane == 0) tma_store_wait_all();
     } else if (landed) {
@@ -339,12 +346,16 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // CTA holds its 128 channels and 128 of the tokens, so a K step brings it 32 KB
 // for 256 x 256 x 128 products (a lone CTA would need 48 KB for half of them,
 // more than L2 can give every SM).  Two accumulator buffers in TMEM: a tile's
-// epilogue runs under the next tile's MMAs.  Warps 0-7 epilogue, 8 TMA
-// producer, 9 MMA (in the leader).
-constexpr int kPairThreads = 320, kPairN = 256;
+// epilogue runs under the next tile's MMAs.  Warps 0-15 epilogue (64 columns of a
+// TMEM lane quarter each: with 8 warps the chain of loads, conversions and
+// stores of a chunk was longer than the MMAs of a tile of small k, 12544 x 256 x
+// 2048 in bf16 22 us, with 16 18.4 us), 16 TMA producer, 17 MMA (in the leader).
+constexpr int kPairN = 256;
+constexpr int kPairEpi = 16, kPairThreads = (kPairEpi + 2) * 32;  // epilogue warps
+constexpr int kPairCols = kPairN * 4 / kPairEpi;  // columns of an epilogue warp
 constexpr int kPairStage = kPBytes + kPairN / 2 * kBK;
-constexpr int pair_stages(int elem) { return elem == 4 ? 5 : 6; }
-constexpr size_t pair_smem(int elem) { return size_t(pair_stages(elem)) * kPairStage + 8 * 2048 * elem + 1024; }
+constexpr int pair_stages(int elem) { return kPairEpi * elem > 32 ? 5 : 6; }
+constexpr size_t pair_smem(int elem) { return size_t(pair_stages(elem)) * kPairStage + size_t(kPairEpi * elem) * 1024 + 1024; }
 
 template <class T>
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -369,12 +380,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accf_bar[b], 1);
-      mbar_init(&acce_bar[b], 16);  // one arrival per epilogue warp of both CTAs
+      mbar_init(&acce_bar[b], 2 * kPairEpi);  // one arrival per epilogue warp of both CTAs
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == kPairEpi + 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -386,9 +397,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  if (warp < 8) {
-    const int quarter = warp & 3, col0 = (warp >> 2) * (kPairN / 2);
-    T *buffers = reinterpret_cast<T *>(smem + STAGES * kPairStage) + warp * 2048;
+  if (warp < kPairEpi) {
+    const int quarter = warp & 3, col0 = (warp >> 2) * kPairCols;
+    T *buffers = reinterpret_cast<T *>(smem + STAGES * kPairStage) + warp * 1024;
     int count = 0;
     for (int ti = 0; ti < my_tiles; ++ti) {
       const int t = tile0 + ti * tstep, ab = ti & 1;
@@ -396,22 +407,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t m0 = int64_t(t / n_tiles) * kPairN;
       const float sw = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
       const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+      float mine[kPairCols / 32];
+#pragma unroll
+      for (int k = 0; k < kPairCols / 32; ++k) mine[k] = token_scale(p, m0 + col0 + k * 32 + lane);
       if (!__all_sync(0xffffffffu, mbar_wait(&accf_bar[ab], (ti >> 1) & 1, &abort_flag, status, 4))) break;
       tc_fence_after();
-#pragma unroll 1
-      for (int c = col0; c < col0 + kPairN / 2; c += 32) {
+#pragma unroll
+      for (int k = 0; k < kPairCols / 32; ++k) {
+        const int c = col0 + k * 32;
         uint32_t acc[32];
         tmem_ld32(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(ab * kPairN + c), acc);
-        if (c + 32 == col0 + kPairN / 2) {
+        if (k == kPairCols / 32 - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_rank_tmem(&acce_bar[ab], 0);
         }
-        if (m0 + c < p.m) store_chunk<T, 32>(p, &ymap, buffers, count, acc, n - lane, m0 + c, lane, sw, bias);
+        if (m0 + c < p.m) store_chunk<T, 32, 1>(p, &ymap, buffers, count, acc, n - lane, m0 + c, lane, mine[k], sw, bias);
       }
     }
     if (lane == 0) tma_store_wait_all();
-  } else if (warp == 8) {
+  } else if (warp == kPairEpi) {
     if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
@@ -467,7 +482,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   __syncwarp();
   cluster_sync();  // the leader's MMAs read the peer's shared memory until here
-  if (warp == 9) {
+  if (warp == kPairEpi + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
@@ -494,17 +509,22 @@ bool encode_y(CUtensorMap *map, const LinearArgs &p) {
                        uint64_t(p.n), uint64_t(p.m), pitch, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Shared memory of a CTA: one with fewer K steps than stages asks for what it
+// uses, so that clusters find room beside one another.
+template <class T>
+size_t split_used(int bn, int num_kb, int csize) {
+  const size_t stages = size_t(std::min(split_stages(bn), int(ceil_div(num_kb, csize)))) * (kPBytes + bn * kBK);
+  return std::max(stages, csize > 1 ? size_t(bn) * kBP * 4 : 4 * 2048 * sizeof(T)) + 1024;
+}
+
 template <class T, int BN>
 int launch_split(const LinearArgs &p, const CUtensorMap &ymap, int n_tiles, int m_tiles, int num_kb, int csize, cudaStream_t s) {
   if (const int rc = allow_smem<linear_split_kernel<T, BN>>(split_smem(BN))) return rc;
   CUtensorMap wmap, amap;
   if (!encode_rows(&wmap, p.w, p.n, p.w_stride, p.k, kBP) || !encode_rows(&amap, p.a, p.m, p.a_stride, p.k, BN))
     return SPKV2_ERR_CUDA;
-  // A CTA with fewer K steps than stages asks for what it uses: less shared
-  // memory, so that clusters find room beside one another.
-  const size_t used = std::max(size_t(std::min(split_stages(BN), int(ceil_div(num_kb, csize)))) * (kPBytes + BN * kBK),
-                               size_t(csize > 1 ? BN * kBP * 4 : 4 * 2048 * int(sizeof(T)))) + 1024;
-  return cuda_status(launch_kernel(linear_split_kernel<T, BN>, unsigned(n_tiles * m_tiles * csize), kSplitThreads, used, s, csize,
+  return cuda_status(launch_kernel(linear_split_kernel<T, BN>, unsigned(n_tiles * m_tiles * csize), kSplitThreads,
+                                   split_used<T>(BN, num_kb, csize), s, csize,
                                    wmap, amap, ymap, p, n_tiles, num_kb, csize));
 }
 
@@ -519,9 +539,17 @@ int launch_pair(const LinearArgs &p, const CUtensorMap &ymap, int n_tiles, int m
                                    s, 2, wmap, amap, ymap, p, n_tiles, tiles, num_kb));
 }
 
-// The cheapest shape by the cycles of its busiest SM: MMA steps (2 cycles for
-// each token column of a K step) or operand bytes (64 a cycle from L2),
-// whichever is more, times the tiles it runs one after another.
+// The cheapest shape by an estimate of its time in microseconds, fitted to
+// measured sweeps over all shapes of some forty sizes (1 .. 12544 tokens, k 93 ..
+// 16000, n 64 .. 16384; the choice took at most 22 % longer than the best one, over
+// most sizes less than 5 %):
+//   single tile: 2.6 launch, 0.7 first operands (once where a CTA leaves room
+//     for a second on its SM), 0.2 a K step (0.28 with 256 columns) while every
+//     SM has one tile and 0.0015 a row of operands beyond, when L2 is the limit;
+//     epilogue 0.1 + 0.015 a column, twice that where y takes no TMA stores; with
+//     a cluster 0.3 + 0.023 a column instead, for the join;
+//   pairs: 2.6 launch, 2.4 for the first operands and the last epilogue, 0.31 a
+//     K step and 0.4 a tile.
 template <class T>
 int launch_tc(LinearArgs p, cudaStream_t s) {
   CUtensorMap ymap = {};
@@ -535,13 +563,16 @@ int launch_tc(LinearArgs p, cudaStream_t s) {
     if (tiles > INT32_MAX / 8) continue;
     for (int c = 1; c <= 8; c *= 2) {
       if (c > 1 && (num_kb < 2 * c || tiles * c > sms)) break;
-      const double step = std::max(2.0 * bn, (kBP + bn) * kBK / 64.0);
-      const double cost = double(ceil_div(tiles * c, sms)) * (1500.0 + ceil_div(num_kb, c) * step + 6.0 * bn) + (c > 1 ? 1000.0 : 0.0);
+      const double kb = double(ceil_div(num_kb, c)), rounds = double(ceil_div(tiles * c, sms));
+      const double step = rounds > 1.0 ? 0.0015 * (kBP + bn) : bn == 256 ? 0.28 : 0.2;
+      const bool roomy = split_used<T>(bn, num_kb, c) <= 110 * 1024;
+      const double end = c > 1 ? 0.3 + 0.023 * bn : (0.1 + 0.015 * bn) * (p.y_tma ? 1.0 : 2.0);
+      const double cost = 2.6 + 0.7 * (roomy ? 1.0 : rounds) + rounds * (kb * step + end);
       if (cost < best) best = cost, best_bn = bn, best_c = c;
     }
   }
   const int64_t pn = ceil_div(p.n, 2 * kBP), pm = ceil_div(p.m, kPairN);
-  const double pair = double(ceil_div(pn * pm, sms / 2)) * num_kb * 512.0 + 4000.0;
+  const double pair = 5.0 + double(ceil_div(pn * pm, sms / 2)) * (num_kb * 0.31 + 0.4);
   if (pn * pm <= INT32_MAX / 2 && (pair < best || !best_bn)) return launch_pair<T>(p, ymap, int(pn), int(pm), num_kb, s);
   const int nt = int(n_tiles), mt = int(ceil_div(p.m, best_bn));
   switch (best_bn) {
