@@ -9,9 +9,7 @@
 // and both reductions (sum of s^2, max |s w|) run in one pass over the row.
 // Quantising without the norm is the same with r = 0, w = 1 and no factor.
 //
-// |s w| is compared by its bits: as an unsigned number, without the sign, a
-// NaN is above infinity and infinity above every finite value, so the
-// maximum itself says whether the row is finite.
+// The maximum keeps a NaN, so it says by itself whether the row is finite.
 #include "transformer.cuh"
 
 namespace spkv2 {
@@ -20,7 +18,8 @@ namespace {
 
 using namespace xf;
 
-constexpr int64_t kMaxWidth = int64_t(1) << 24;
+constexpr int64_t kMaxWidth = int64_t(1) << 24, kMostWidth = 16384;  // of a call; of rows kept in registers
+constexpr int kPerThread = 16;  // elements; with 8 the synchronisation costs more (40000 x 512 in bf16: 29 us, with 16 24 us)
 
 struct RowArgs {
   const void *x, *residual, *weight;
@@ -32,10 +31,16 @@ struct RowArgs {
   float eps;
 };
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The larger of two magnitudes; a NaN stays.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-// The factor that takes |s w| to codes.  127 / amax overflows where amax is
-// below 2^-121 or so; values that small are scaled up by 2^64, exactly, first.
+// What takes s w to codes: code = rne(v * pre * inv).  127 / amax overflows where
+// amax is below 2^-121 or so; values that small are scaled up by pre = 2^64,
+// exactly, first.  Both are 0 for rows of zeros and rows that are not finite.
 struct CodeScale {
   float pre, inv;
 };
@@ -45,7 +50,13 @@ __device__ __forceinline__ CodeScale code_scale(float amax) {
   c.inv = amax > 0.0f ? 127.0f / (amax * c.pre) : 0.0f;
   return c;
 }
-__device__ __forceinline__ int8_t code_of(float v, CodeScale c) { return sat_rne_i8(v * c.pre * c.inv, -127); }
+// |v| <= amax, so v * inv rounds to at most 127 in magnitude, and adding 1.5 * 2^23
+// rounds it to the nearest even integer, which lands in the sum's low byte in
+// two's complement.
+__device__ __forceinline__ uint32_t code_bits(float v, float inv) { return __float_as_uint(fmaf(v, inv, 12582912.0f)); }
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
 // N elements in one access.
 template <class T, int N>
@@ -53,11 +64,50 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 
+// 16 bytes of elements as fp32 and back, two elements of 16 bits a step: taken one
+// by one out of a struct they cost a row kernel three times the instructions.
+__device__ __forceinline__ void expand(const uint4 &u, float (&f)[4], float) {
+  f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void expand(const uint4 &u, float (&f)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void expand(const uint4 &u, float (&f)[8], __half) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    f[2 * i] = v.x, f[2 * i + 1] = v.y;
+  }
+}
+__device__ __forceinline__ uint4 contract(const float (&f)[4], float) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 contract(const float (&f)[8], __nv_bfloat16) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 contract(const float (&f)[8], __half) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A row's scale (its first thread writes it) and the factor of its codes.
 template <bool NORM>
-__device__ __forceinline__ CodeScale finish_row(const RowArgs &p, int64_t row, float ss, uint32_t mx, bool &finite, bool writes) {
-  finite = mx < 0x7f800000u;
-  const float amax = __uint_as_float(mx);
+__device__ __forceinline__ CodeScale finish_row(const RowArgs &p, int64_t row, float ss, float amax, bool &finite, bool writes) {
+  finite = amax < INFINITY;
   if (writes) {
     const float f = NORM && amax > 0.0f ? 1.0f / sqrtf(ss / float(p.width) + p.eps) : 1.0f;
     p.scale[row] = finite ? amax * f / 127.0f : __uint_as_float(0x7fc00000u);
@@ -65,116 +115,159 @@ __device__ __forceinline__ CodeScale finish_row(const RowArgs &p, int64_t row, f
   return code_scale(finite ? amax : 0.0f);
 }
 
-// Bound by memory: every element is read once, kept in registers (EPT a thread)
-// through the row's two reductions, and its code written once.  A thread owns
-// units of 16 bytes of x (U elements), t, t + tpr, ..: which element is added
-// where does not depend on alignment, so neither do the bits of the result.
+__host__ __device__ __forceinline__ int stage_at(int e, int u) { return e + e / u; }
+__host__ __device__ __forceinline__ int stage_floats(int width, int u) { return stage_at((width + u - 1) / u * u, u); }
+
+// Bound by memory: every element is read once, kept in registers (16 a thread)
+// through the row's two reductions, and its code written once.  A block for each
+// row (or a few) and no more: blocks that stay, load the next row ahead and keep
+// the weights need registers that cost more loads in flight than they save
+// (16384 x 4096 in bf16: 147 us, without 96 us).
+//
+// A thread owns units of 16 bytes of x (U elements), t, t + tpr, ..: which element
+// is added where depends on the width alone, not on alignment or the number of
+// rows, so neither do the bits of the result.
 //
 // STAGED: rows that do not start on 16-byte boundaries, or end inside a unit.
-// They are read element by element in order, a warp's 32 side by side, and pass
-// through shared memory (as fp32 sums) to the threads that own them; reading the
-// units themselves element by element would touch each line eight times.
+// They are read in the 16-byte pieces that memory has, and pass through shared
+// memory (as fp32 sums) to the threads that own the units.  One word of padding a
+// unit: a warp's accesses to the same place of 32 units fall into 32 banks.
 //
 // The residual's sum is written by the thread that read both parts, so it may
-// take their place.  tpr (32 .. 1024, a power of two) threads a row; rows of less
-// than 128 threads share a block.
-template <class T, bool NORM, int EPT, bool STAGED>
-__global__ void __launch_bounds__(1024) row_codes_kernel(RowArgs p, int tpr, bool vec_codes) {
-  constexpr int U = 16 / sizeof(T), N = EPT / U;
+// take their place.  rpb rows a block: one row of any number of warps, or several
+// of a power of two of threads.
+template <class T, bool NORM, bool STAGED>
+__global__ void __launch_bounds__(1024)
+    row_codes_kernel(RowArgs p, int tpr, int rpb, bool vec_codes, bool vec_weight) {
+  constexpr int U = 16 / sizeof(T), N = kPerThread / U;
   extern __shared__ __align__(16) float staged[];
-  __shared__ float s_sum[32];
-  __shared__ uint32_t s_max[32];
+  __shared__ float s_sum[32], s_max[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = threadIdx.x & (tpr - 1), wpr = tpr >> 5;
-  const int64_t row = int64_t(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-  const bool real = row < p.rows;
+  const int sub = rpb > 1 ? threadIdx.x / tpr : 0, t = threadIdx.x - sub * tpr, wpr = tpr >> 5;
   const int width = int(p.width);
+  const T *w = static_cast<const T *>(p.weight);
+  float *mine = staged + sub * stage_floats(width, U);
+
+  auto weights = [&](int c) {
+    Vec<T, U> wv;
+    if (!STAGED || (vec_weight && c + U <= width)) wv = *reinterpret_cast<const Vec<T, U> *>(w + c);
+    else
+#pragma unroll
+      for (int e = 0; e < U; ++e) wv.v[e] = c + e < width ? w[c + e] : from_f32<T>(0.0f);
+    return *reinterpret_cast<const uint4 *>(&wv);
+  };
+  // A row's pieces: `head` elements before its first 16-byte boundary, whole
+  // units, and the rest from `tail` on.  Where the residual or the sum have their
+  // boundaries elsewhere, all elements count as head.
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  uint4 xv[N], rv[N], wv[N];
+  T xe, re;
+  int head = 0, units = (width + U - 1) / U, tail = width;
+  const int64_t row = int64_t(blockIdx.x) * rpb + sub;
+  const bool real = row < p.rows;
   const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
   const T *r = static_cast<const T *>(p.residual) + row * p.residual_stride;
-  const T *w = static_cast<const T *>(p.weight);
   T *sum = static_cast<T *>(p.sum) + row * p.sum_stride;
-  float v[N][U];
-  float ss = 0.0f;
-  uint32_t mx = 0;
-  if (STAGED) {
-    float *mine = staged + threadIdx.x / tpr * ((width + U - 1) / U * U);
-    constexpr int B = 8;  // loads in flight
-    for (int c0 = t; real && c0 < width; c0 += B * tpr) {
-      float s[B];
-#pragma unroll
-      for (int k = 0; k < B; ++k) s[k] = c0 + k * tpr < width ? to_f32(x[c0 + k * tpr]) : 0.0f;
-      if (NORM && p.residual) {
-#pragma unroll
-        for (int k = 0; k < B; ++k) s[k] += c0 + k * tpr < width ? to_f32(r[c0 + k * tpr]) : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < B; ++k) {
-        const int c = c0 + k * tpr;
-        if (c >= width) break;
-        if (NORM && p.sum) sum[c] = from_f32<T>(s[k]);
-        mine[c] = s[k];
+  if (real) {
+    if (STAGED) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+      const uintptr_t sum_at = reinterpret_cast<uintptr_t>(sum);
+      const bool same = !NORM || ((!p.residual || ((at ^ reinterpret_cast<uintptr_t>(r)) & 15) == 0) &&
+                                  (!p.sum || ((at ^ sum_at) & 15) == 0));
+      head = same ? min(int((16 - (at & 15)) & 15) / int(sizeof(T)), width) : width;
+      units = (width - head) / U;
+      tail = head + units * U;
+      if (t < head + width - tail) {
+        const int e = t < head ? t : t - head + tail;
+        xe = x[e];
+        if (NORM && p.residual) re = r[e];
       }
     }
-    if (real && t < (width + U - 1) / U * U - width) mine[width + t] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int k = t + i * tpr;
+    const bool in = real && k < units;
+    xv[i] = in ? *reinterpret_cast<const uint4 *>(x + head + k * U) : none;
+    if (NORM && p.residual) rv[i] = in ? *reinterpret_cast<const uint4 *>(r + head + k * U) : none;
+  }
+  if (NORM) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) wv[i] = (t + i * tpr) * U < width ? weights((t + i * tpr) * U) : none;
+  }
+  float v[N][U];
+  if (STAGED) {
+    if (real) {
+      for (int c = t; c < head + width - tail; c += tpr) {
+        const int e = c < head ? c : c - head + tail;
+        float s;
+        if (c == t) {
+          s = to_f32(xe);
+          if (NORM && p.residual) s += to_f32(re);
+        } else {
+          s = to_f32(x[e]);
+          if (NORM && p.residual) s += to_f32(r[e]);
+        }
+        if (NORM && p.sum) sum[e] = from_f32<T>(s);
+        mine[stage_at(e, U)] = s;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int k = t + i * tpr;
+        if (k >= units) break;
+        float s[U];
+        expand(xv[i], s, T{});
+        if (NORM && p.residual) {
+          float add[U];
+          expand(rv[i], add, T{});
+#pragma unroll
+          for (int e = 0; e < U; ++e) s[e] += add[e];
+        }
+#pragma unroll
+        for (int e = 0; e < U; ++e) mine[stage_at(head + k * U + e, U)] = s[e];
+        if (NORM && p.sum) *reinterpret_cast<uint4 *>(sum + head + k * U) = contract(s, T{});
+      }
+      if (t < (width + U - 1) / U * U - width) mine[stage_at(width + t, U)] = 0.0f;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = (t + i * tpr) * U;
 #pragma unroll
-      for (int e = 0; e < U; e += 4) {
-        const float4 f = real && c < width ? *reinterpret_cast<const float4 *>(mine + c + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        v[i][e] = f.x, v[i][e + 1] = f.y, v[i][e + 2] = f.z, v[i][e + 3] = f.w;
-      }
+      for (int e = 0; e < U; ++e) v[i][e] = real && c < width ? mine[stage_at(c + e, U)] : 0.0f;
     }
   } else {
-    Vec<T, U> xv[N], rv[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = (t + i * tpr) * U;
-      if (real && c < width) {
-        xv[i] = *reinterpret_cast<const Vec<T, U> *>(x + c);
-        if (NORM && p.residual) rv[i] = *reinterpret_cast<const Vec<T, U> *>(r + c);
-      }
-    }
+      expand(xv[i], v[i], T{});
+      if (NORM && p.residual) {
+        float add[U];
+        expand(rv[i], add, T{});
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (t + i * tpr) * U;
-      const bool in = real && c < width;
-      Vec<T, U> sv;
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        float s = in ? to_f32(xv[i].v[e]) : 0.0f;
-        if (NORM && p.residual && in) s += to_f32(rv[i].v[e]);
-        if (NORM) sv.v[e] = from_f32<T>(s);
-        v[i][e] = s;
+        for (int e = 0; e < U; ++e) v[i][e] += add[e];
       }
-      if (NORM && p.sum && in) *reinterpret_cast<Vec<T, U> *>(sum + c) = sv;
+      if (NORM && p.sum && real && c < width) *reinterpret_cast<uint4 *>(sum + c) = contract(v[i], T{});
     }
   }
+  float ss = 0.0f, mx = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = (t + i * tpr) * U;
-    if (NORM && real && c < width) {
-      Vec<T, U> wv;
-      if (STAGED) {
-#pragma unroll
-        for (int e = 0; e < U; ++e) wv.v[e] = c + e < width ? w[c + e] : from_f32<T>(0.0f);
-      } else {
-        wv = *reinterpret_cast<const Vec<T, U> *>(w + c);
-      }
+  for (int i = 0; i < N; ++i) {  // units past the width hold zeros
+    if (NORM) {
+      float wf[U];
+      expand(wv[i], wf, T{});
 #pragma unroll
       for (int e = 0; e < U; ++e) {
         ss = fmaf(v[i][e], v[i][e], ss);
-        v[i][e] *= to_f32(wv.v[e]);
+        v[i][e] *= wf[e];
       }
     }
 #pragma unroll
-    for (int e = 0; e < U; ++e) mx = max(mx, abs_bits(v[i][e]));
+    for (int e = 0; e < U; ++e) mx = max_nan(mx, fabsf(v[i][e]));
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
+  for (int o = min(tpr, 32) / 2; o; o >>= 1) {
     if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (wpr > 1) {
     if (lane == 0) {
@@ -182,61 +275,68 @@ __global__ void __launch_bounds__(1024) row_codes_kernel(RowArgs p, int tpr, boo
       s_max[warp] = mx;
     }
     __syncthreads();
-    const int first = warp & ~(wpr - 1);
-    ss = lane < wpr ? s_sum[first + lane] : 0.0f;
-    mx = lane < wpr ? s_max[first + lane] : 0;
+    const int w0 = sub * wpr;
+    ss = lane < wpr ? s_sum[w0 + lane] : 0.0f;
+    mx = lane < wpr ? s_max[w0 + lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
   }
   if (!real) return;
   bool finite;
   const CodeScale cs = finish_row<NORM>(p, row, ss, mx, finite, t == 0);
   int8_t *codes = p.codes + row * p.codes_stride;
+  if (cs.pre != 1.0f || !finite) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < U; ++e) v[i][e] = finite ? v[i][e] * cs.pre : 0.0f;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = (t + i * tpr) * U;
     if (c >= width) break;
-    Vec<int8_t, U> q;
+    uint32_t q[U / 4];
 #pragma unroll
-    for (int e = 0; e < U; ++e) q.v[e] = finite ? code_of(v[i][e], cs) : int8_t(0);
+    for (int e = 0; e < U; e += 4)
+      q[e / 4] = pack4(code_bits(v[i][e], cs.inv), code_bits(v[i][e + 1], cs.inv), code_bits(v[i][e + 2], cs.inv),
+                       code_bits(v[i][e + 3], cs.inv));
     if (!STAGED || (vec_codes && c + U <= width)) {
-      *reinterpret_cast<Vec<int8_t, U> *>(codes + c) = q;
+      *reinterpret_cast<Vec<uint32_t, U / 4> *>(codes + c) = *reinterpret_cast<Vec<uint32_t, U / 4> *>(q);
     } else {
 #pragma unroll
       for (int e = 0; e < U; ++e)
-        if (c + e < width) codes[c + e] = q.v[e];
+        if (c + e < width) codes[c + e] = int8_t(q[e / 4] >> (8 * (e & 3)));
     }
   }
 }
 
-// Rows wider than the registers of a block (32 elements a thread): one block a
-// row, which is read twice, the second time from L2; the sum is written in the
+// Rows wider than kMostWidth, the registers of a block: one block a row, which is read twice, the second time from L2; the sum is written in the
 // second pass, as it may take x's or the residual's place.
 template <class T, bool NORM>
 __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
   __shared__ float s_sum[32];
-  __shared__ uint32_t s_max[32];
+  __shared__ float s_max[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int64_t row = blockIdx.x;
   const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
   const T *r = NORM && p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
   const T *w = static_cast<const T *>(p.weight);
   float ss = 0.0f;
-  uint32_t mx = 0;
+  float mx = 0.0f;
 #pragma unroll 4
   for (int64_t i = tid; i < p.width; i += threads) {
     float s = to_f32(x[i]);
     if (r) s += to_f32(r[i]);
     ss = fmaf(s, s, ss);
-    mx = max(mx, abs_bits(NORM ? s * to_f32(w[i]) : s));
+    mx = max_nan(mx, fabsf(NORM ? s * to_f32(w[i]) : s));
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (lane == 0) {
     s_sum[warp] = ss;
@@ -248,7 +348,7 @@ __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   bool finite;
   const CodeScale c = finish_row<NORM>(p, row, ss, mx, finite, tid == 0);
@@ -258,7 +358,7 @@ __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
   for (int64_t i = tid; i < p.width; i += threads) {
     float s = to_f32(x[i]);
     if (r) s += to_f32(r[i]);
-    codes[i] = finite ? code_of(NORM ? s * to_f32(w[i]) : s, c) : int8_t(0);
+    codes[i] = finite ? int8_t(code_bits((NORM ? s * to_f32(w[i]) : s) * c.pre, c.inv)) : int8_t(0);
     if (sum) sum[i] = from_f32<T>(s);
   }
 }
@@ -284,26 +384,51 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <class T, bool NORM, int EPT, bool STAGED>
-int launch_ept(const RowArgs &a, int tpr, bool vec_codes, cudaStream_t s) {
-  const int threads = std::max(tpr, 128), rpb = threads / tpr;
+// The same where rows of y do not lie on 16-byte boundaries, or end inside one: a
+// thread writes the 16 bytes between two boundaries (or, first and last in a row,
+// what there is of them) from codes that start anywhere.
+template <class T>
+__global__ void __launch_bounds__(256)
+    row_values_shifted_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, int width,
+                              uint32_t chunks, FastDiv per_row, int64_t codes_stride, int64_t y_stride) {
   constexpr int U = 16 / sizeof(T);
-  const size_t smem = STAGED ? size_t(rpb) * (size_t(a.width) + U - 1) / U * U * 4 : 0;
-  if (STAGED)
-    if (const int rc = allow_smem<row_codes_kernel<T, NORM, EPT, STAGED>>(32768 * 4)) return rc;
-  row_codes_kernel<T, NORM, EPT, STAGED><<<unsigned(ceil_div(a.rows, rpb)), threads, smem, s>>>(a, tpr, vec_codes);
-  return cuda_status(cudaGetLastError());
+  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < chunks; i += gridDim.x * 256u) {
+    const uint32_t row = per_row.div(i), k = i - row * per_row.d;
+    T *to = y + int64_t(row) * y_stride;
+    const int8_t *from = codes + int64_t(row) * codes_stride;
+    const int head = int((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / int(sizeof(T));
+    const int c = k == 0 ? 0 : head + int(k - 1) * U, end = min(k == 0 ? head : c + U, width);
+    if (c >= end) continue;
+    const float s = __ldg(scale + row);
+    if (k > 0 && c + U <= width) {
+      Vec<T, U> o;
+#pragma unroll
+      for (int e = 0; e < U; ++e) o.v[e] = from_f32<T>(float(from[c + e]) * s);
+      *reinterpret_cast<Vec<T, U> *>(to + c) = o;
+    } else {
+      for (int e = c; e < end; ++e) to[e] = from_f32<T>(float(from[e]) * s);
+    }
+  }
 }
 
 template <class T, bool NORM, bool STAGED>
 int launch_row(const RowArgs &a, bool vec_codes, cudaStream_t s) {
-  // Eight elements a thread for rows of one block's 256 threads, 16 beyond (less
-  // synchronisation for the same loads in flight), 32 where 1024 threads need them.
-  const int64_t per = a.width <= 2048 ? 8 : a.width <= 16384 ? 16 : 32;
-  int tpr = 32;
-  while (tpr * per < a.width) tpr *= 2;
-  if (per == 8) return launch_ept<T, NORM, 8, STAGED>(a, tpr, vec_codes, s);
-  return per == 16 ? launch_ept<T, NORM, 16, STAGED>(a, tpr, vec_codes, s) : launch_ept<T, NORM, 32, STAGED>(a, tpr, vec_codes, s);
+  constexpr auto kern = row_codes_kernel<T, NORM, STAGED>;
+  constexpr int U = 16 / sizeof(T);
+  // One row of as many warps as it needs, or several of a power of two of threads.
+  int tpr = int(ceil_div(ceil_div(a.width, U), kPerThread / U)), rpb = 1;
+  if (tpr <= 64) {
+    int up = 8;
+    while (up < tpr) up *= 2;
+    tpr = up, rpb = 128 / up;
+  } else {
+    tpr = (tpr + 31) / 32 * 32;
+  }
+  const size_t smem = STAGED ? size_t(rpb) * stage_floats(int(a.width), U) * 4 : 0;
+  if (STAGED)
+    if (const int rc = allow_smem<kern>(stage_floats(kMostWidth, U) * 4)) return rc;
+  kern<<<unsigned(ceil_div(a.rows, rpb)), tpr * rpb, smem, s>>>(a, tpr, rpb, vec_codes, aligned16(a.weight));
+  return cuda_status(cudaGetLastError());
 }
 
 // The most elements (a power of two up to `most`) that rows can be accessed by:
@@ -319,7 +444,7 @@ template <bool NORM>
 int launch_rows(const RowArgs &a, int32_t dtype, cudaStream_t s) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.width > 32768) {
+    if (a.width > kMostWidth) {
       wide_codes_kernel<T, NORM><<<unsigned(a.rows), 1024, 0, s>>>(a);
       return cuda_status(cudaGetLastError());
     }
@@ -385,16 +510,19 @@ extern "C" int spkv2_cuda_dequantize_rows_i8(const Spkv2DequantizeRowsI8 *a, voi
     // Stores of 16 bytes at most: y's alignment beyond them does not matter.
     constexpr int64_t size = sizeof(T);
     const bool many = a->rows > 1;
-    int vw = vector_width(16, a->width, reinterpret_cast<uintptr_t>(a->codes), many ? a->codes_stride : 0);
+    const int vw = vector_width(16, a->width, reinterpret_cast<uintptr_t>(a->codes), many ? a->codes_stride : 0);
     const int vy = vector_width(16 / int(size), a->width, reinterpret_cast<uintptr_t>(a->y) / size, many ? a->y_stride : 0);
-    if (vy < 16 / int(size)) vw = std::min(vw, vy);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch (vw) {
-      case 16: return launch_values<T, 16>(a, s);
-      case 8: return launch_values<T, 8>(a, s);
-      case 4: return launch_values<T, 4>(a, s);
-      case 2: return launch_values<T, 2>(a, s);
-      default: return launch_values<T, 1>(a, s);
+    if (std::min(vw, vy) < 16 / int(size)) {
+      const int64_t per_row = 1 + ceil_div(a->width, 16 / size), chunks = per_row * a->rows;
+      if (chunks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+      row_values_shifted_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64)), 256, 0, s>>>(
+          a->codes, a->scale, static_cast<T *>(a->y), int(a->width), uint32_t(chunks), FastDiv(uint32_t(per_row)),
+          a->codes_stride, a->y_stride);
+      return cuda_status(cudaGetLastError());
     }
+    if (vw == 16) return launch_values<T, 16>(a, s);
+    if (size == 2 || vw == 8) return launch_values<T, 8>(a, s);
+    return launch_values<T, 4>(a, s);
   });
 }
