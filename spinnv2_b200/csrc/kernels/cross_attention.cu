@@ -20,39 +20,64 @@ namespace spkv2 {
 namespace {
 
 using namespace xf;
+using namespace tc;
 
 // ------------------------------------------------------------ CUDA cores
-// Any type, width and alignment, exact fp32 products.  64 rows x 64 keys a
-// step, 256 threads; a thread holds scores for 4 rows x 4 keys and sums for
-// 4 rows x D / 16 columns.  The 16 threads of a row group are half a warp.
-constexpr int kRows = 64, kKeys = 64;
+// Any type, width and alignment, exact fp32 products.  16 R rows x 64 keys a
+// step, 256 threads; a thread holds scores for R rows x 4 keys and sums for R
+// rows x D / 16 columns.  The 16 threads of a row group are half a warp.  Bound
+// by the FMA pipe with four rows a thread (their operands take 12 of 16
+// shared-memory cycles); with few rows by shared memory, which every warp reads
+// whole for its two rows.  With too few row tiles for the SMs the CTAs of a
+// cluster divide the keys and join their m, l and O through distributed shared
+// memory, in CTA order.
+constexpr int kKeys = 64, kMaxCluster = 8;
 
-template <int D>
+template <int D, int R>
 struct SimtSmem {
-  float q[kRows][D + 4];
-  float k[kKeys][D + 4];
+  static constexpr int rows = 16 * R;
+  float k[kKeys][D + 4];  // at the end O, [row][D]
   float v[kKeys][D];
-  float p[kRows][kKeys + 4];
+  float q[rows][D + 4];
+  float p[rows][kKeys + 4];
+  float m[rows], l[rows];
   int valid[kKeys];
 };
 
-template <class T, int D>
-__global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
+// Four elements of a row as fp32, in one access.
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+template <class T>
+__device__ __forceinline__ float4 load4(const T *p) {
+  const uint2 u = *reinterpret_cast<const uint2 *>(p);
+  const T *e = reinterpret_cast<const T *>(&u);
+  return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
+}
+
+template <class T, int D, int R>
+__global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a, int csize, bool vec) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  SimtSmem<D> &sm = *reinterpret_cast<SimtSmem<D> *>(smem_raw);
+  using S = SimtSmem<D, R>;
+  S &sm = *reinterpret_cast<S *>(smem_raw);
+  static_assert(S::rows <= kKeys, "O takes the place of the keys");
   constexpr int CPT = D / 16;  // columns of a thread: tx * CW + 16 * CW * c
   constexpr int CW = CPT < 4 ? CPT : 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  int t = blockIdx.x;
-  const int r0 = t % a.row_tiles * kRows;
+  const int rank = csize > 1 ? int(cluster_rank()) : 0;
+  int t = int(blockIdx.x) / csize;
+  const int r0 = t % a.row_tiles * S::rows;
   t /= a.row_tiles;
   const int hk = t % a.kv_heads, b = t / a.kv_heads;
   const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
   const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
   const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  const int keys = entry_keys(a, b);
+  const int keys = entry_keys(a, b), tiles = (keys + kKeys - 1) / kKeys;
+  const int tile0 = int(int64_t(tiles) * rank / csize), tile1 = int(int64_t(tiles) * (rank + 1) / csize);
+  auto out_row = [&](int row) {
+    const int qi = row / a.group, h = hk * a.group + row % a.group;
+    return static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+  };
 
-  for (int e = tid; e < kRows * D; e += 256) {
+  for (int e = tid; e < S::rows * D; e += 256) {
     const int r = e / D, c = e % D, row = r0 + r;
     float val = 0.0f;
     if (row < a.rows && c < a.width) {
@@ -61,35 +86,47 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
     }
     sm.q[r][c] = val;
   }
-  float o[4][CPT] = {}, m[4], l[4] = {};
+  float o[R][CPT] = {}, m[R], l[R] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
+  for (int i = 0; i < R; ++i) m[i] = -INFINITY;
 
-  for (int j0 = 0; j0 < keys; j0 += kKeys) {
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int j0 = tile * kKeys;
     __syncthreads();  // the last tile's readers are done
     if (tid < kKeys) {
       const int j = j0 + tid;
       sm.valid[tid] = j < keys && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
     }
     __syncthreads();
-    for (int e = tid; e < kKeys * D; e += 256) {
-      const int r = e / D, c = e % D;
-      const bool in = sm.valid[r] && c < a.width;
-      sm.k[r][c] = in ? to_f32(k[(j0 + r) * a.ks[1] + c]) : 0.0f;
-      sm.v[r][c] = in ? to_f32(v[(j0 + r) * a.vs[1] + c]) : 0.0f;
+    if (vec) {
+#pragma unroll 4
+      for (int e = tid * 4; e < kKeys * D; e += 1024) {
+        const int r = e / D, c = e % D;
+        const bool in = sm.valid[r] && c < a.width;
+        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<float4 *>(&sm.k[r][c]) = in ? load4(k + (j0 + r) * a.ks[1] + c) : zero;
+        *reinterpret_cast<float4 *>(&sm.v[r][c]) = in ? load4(v + (j0 + r) * a.vs[1] + c) : zero;
+      }
+    } else {
+#pragma unroll 4
+      for (int e = tid; e < kKeys * D; e += 256) {
+        const int r = e / D, c = e % D;
+        const bool in = sm.valid[r] && c < a.width;
+        sm.k[r][c] = in ? to_f32(k[(j0 + r) * a.ks[1] + c]) : 0.0f;
+        sm.v[r][c] = in ? to_f32(v[(j0 + r) * a.vs[1] + c]) : 0.0f;
+      }
     }
     __syncthreads();
-    float s[4][4] = {};
+    float s[R][4] = {};
 #pragma unroll 4
     for (int c = 0; c < D; c += 4) {
-      float4 qv[4], kv[4];
+      float4 qv[R], kv[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        qv[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * 4 + i][c]);
-        kv[i] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * i][c]);
-      }
+      for (int i = 0; i < R; ++i) qv[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * R + i][c]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * j][c]);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
@@ -99,7 +136,7 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
       float mx = m[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -116,7 +153,7 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
       for (int j = 0; j < 4; ++j) {
         const float e = exp2f(s[i][j] - use);
         sum += e;
-        sm.p[ty * 4 + i][tx + 16 * j] = e;
+        sm.p[ty * R + i][tx + 16 * j] = e;
       }
       l[i] = l[i] * shrink + sum;  // this thread's keys only; joined at the end
 #pragma unroll
@@ -125,9 +162,9 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
     __syncwarp();  // a row's 16 threads are in one warp
 #pragma unroll 2
     for (int j = 0; j < kKeys; j += 4) {
-      float4 pv[4];
+      float4 pv[R];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4 *>(&sm.p[ty * 4 + i][j]);
+      for (int i = 0; i < R; ++i) pv[i] = *reinterpret_cast<const float4 *>(&sm.p[ty * R + i][j]);
 #pragma unroll
       for (int jj = 0; jj < 4; ++jj) {
 #pragma unroll
@@ -136,7 +173,7 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
 #pragma unroll
           for (int w = 0; w < CW; ++w) vv[w] = sm.v[j + jj][tx * CW + 16 * c + w];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < R; ++i) {
             const float e = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w;
 #pragma unroll
             for (int w = 0; w < CW; ++w) o[i][c + w] = fmaf(e, vv[w], o[i][c + w]);
@@ -146,31 +183,93 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float sum = l[i];
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    const int row = r0 + ty * 4 + i;
-    if (row >= a.rows) continue;
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    const int qi = row / a.group, h = hk * a.group + row % a.group;
-    T *out = static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+    for (int w = 8; w; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+  if (csize == 1) {
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-      const int col = tx * CW + 16 * (c / CW * CW) + c % CW;
-      if (col < a.width) out[col] = from_f32<T>(o[i][c] * inv);
+    for (int i = 0; i < R; ++i) {
+      const int row = r0 + ty * R + i;
+      if (row >= a.rows) continue;
+      const float inv = l[i] != 0.0f ? 1.0f / l[i] : 0.0f;
+      T *out = out_row(row);
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        const int col = tx * CW + 16 * (c / CW * CW) + c % CW;
+        if (col < a.width) out[col] = from_f32<T>(o[i][c] * inv);
+      }
+    }
+    return;
+  }
+  __syncthreads();  // the last tile's readers are done: O takes the keys' place
+  float *part = &sm.k[0][0];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) part[(ty * R + i) * D + tx * CW + 16 * (c / CW * CW) + c % CW] = o[i][c];
+    if (tx == 0) {
+      sm.m[ty * R + i] = m[i];
+      sm.l[ty * R + i] = l[i];
     }
   }
+  cluster_sync();
+  const int used = min(S::rows, a.rows - r0) * D;
+  for (int e = rank * 256 + tid; e < used; e += csize * 256) {
+    const int r = e / D, c = e % D;
+    float mk[kMaxCluster], lk[kMaxCluster], ok[kMaxCluster], top = -INFINITY, acc = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kMaxCluster; ++n) {
+      if (n >= csize) break;
+      mk[n] = __uint_as_float(ld_cluster(map_rank(&sm.m[r], n)));
+      lk[n] = __uint_as_float(ld_cluster(map_rank(&sm.l[r], n)));
+      ok[n] = __uint_as_float(ld_cluster(map_rank(&part[e], n)));
+      top = fmaxf(top, mk[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < kMaxCluster; ++n) {
+      if (n >= csize) break;
+      const float f = mk[n] == -INFINITY ? 0.0f : exp2f(mk[n] - top);
+      acc = fmaf(ok[n], f, acc);
+      sum = fmaf(lk[n], f, sum);
+    }
+    if (c < a.width) out_row(r0 + r)[c] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+  }
+  cluster_sync();  // the peers have read this CTA's sums
 }
 
-template <class T, int D>
+template <class T, int D, int R>
 int launch_simt(AttnArgs a, cudaStream_t s) {
-  a.row_tiles = int(ceil_div(a.rows, kRows));
+  using S = SimtSmem<D, R>;
+  a.row_tiles = int(ceil_div(a.rows, S::rows));
   const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
-  if (blocks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  if (const int rc = allow_smem<cross_simt_kernel<T, D>>(sizeof(SimtSmem<D>))) return rc;
-  cross_simt_kernel<T, D><<<unsigned(blocks), 256, sizeof(SimtSmem<D>), s>>>(a);
-  return cuda_status(cudaGetLastError());
+  if (const int rc = allow_smem<cross_simt_kernel<T, D, R>>(sizeof(S))) return rc;
+  auto fours = [](const void *base, const int64_t (&st)[3]) {
+    return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+  };
+  const bool vec = a.width % 4 == 0 && fours(a.k, a.ks) && fours(a.v, a.vs);
+  // Divide the keys while a CTA keeps a tile and the CTAs are fewer than two an SM.
+  int csize = 1;
+  while (csize < kMaxCluster && blocks * csize * 2 <= 2 * sm_count() && ceil_div(a.keys, kKeys) >= 2 * csize) csize *= 2;
+  if (blocks * csize > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  // Without programmatic launch: the kernel reads global memory from its start.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks * csize));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = sizeof(S);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(csize);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = csize > 1 ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, cross_simt_kernel<T, D, R>, a, csize, vec));
+}
+
+// Sixteen rows a tile where they are all there are, else 64.
+template <class T, int D>
+int launch_rows(const AttnArgs &a, cudaStream_t s) {
+  return a.rows <= 16 ? launch_simt<T, D, 1>(a, s) : launch_simt<T, D, 4>(a, s);
 }
 
 }  // namespace
@@ -208,9 +307,9 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   if (cross_tc_serves(a, x->dtype)) return a.rows <= 32 ? cross_step(a, x->dtype, s) : cross_tc(a, x->dtype, s);
   return by_type(x->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.width <= 32) return launch_simt<T, 32>(a, s);
-    if (a.width <= 64) return launch_simt<T, 64>(a, s);
-    if (a.width <= 128) return launch_simt<T, 128>(a, s);
-    return launch_simt<T, 256>(a, s);
+    if (a.width <= 32) return launch_rows<T, 32>(a, s);
+    if (a.width <= 64) return launch_rows<T, 64>(a, s);
+    if (a.width <= 128) return launch_rows<T, 128>(a, s);
+    return launch_rows<T, 256>(a, s);
   });
 }
