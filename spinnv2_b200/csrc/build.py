@@ -3,6 +3,8 @@
 Every .cu/.cpp under csrc/ is compiled by nvcc for sm_100a only and linked
 into spinnv2_b200/_lib/libspkv2_runtime.so together with the static CUDA
 runtime, so the library needs nothing but the NVIDIA driver at load time.
+build_binding() compiles the torch binding of the decoder-layer operators
+beside it (_lib/_torch_ops.so), with g++ against the installed torch.
 Objects are rebuilt when a source or any header under csrc/ or include/
 is newer than the object.
 """
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -23,6 +26,8 @@ INCLUDE = REPO_DIR / "include"
 BUILD_DIR = REPO_DIR / "_build" / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libspkv2_runtime.so"
+BINDING_SOURCE = PKG_DIR / "binding" / "torch_ops.cpp"
+BINDING_PATH = LIB_DIR / "_torch_ops.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = [
@@ -93,6 +98,28 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     return LIB_PATH
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the torch binding of the decoder-layer operators (a CPython module for the
+    interpreter and the torch that run this)."""
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    if BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= max(
+            p.stat().st_mtime for p in (BINDING_SOURCE, INCLUDE / "spkv2_transformer.h")):
+        return BINDING_PATH
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    includes = [INCLUDE, sysconfig.get_path("include"), Path(_nvcc()).parent.parent / "include", *include_paths()]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(f"-I{p}" for p in includes),
+           str(BINDING_SOURCE), "-o", str(BINDING_PATH), *(f"-L{p}" for p in library_paths()),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SOURCE.name}:\n{res.stdout}\n{res.stderr}")
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
     path = build(verbose="-v" in sys.argv)
     print(path)
+    print(build_binding(verbose="-v" in sys.argv))

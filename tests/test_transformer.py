@@ -6,7 +6,11 @@ few multiples of 2^-24 per operation, summed sizes included.
 
 from __future__ import annotations
 
+import ctypes
 import math
+import struct
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -509,28 +513,39 @@ def test_refusals(gpu):
     assert e.value.code == -43
 
 
+# The argument structs of spkv2_transformer.h, in native alignment.
+NORM, CODES, LINEAR_ARGS, CROSS = (struct.Struct(f) for f in ("@6P6qfi", "@3P4qii", "@6P6qii", "@6P16q4ifi"))
+
+
+def c_function(name):
+    from spinnv2_b200.runtime import load_library
+
+    fn = getattr(load_library(), name)
+    fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
+    return fn
+
+
 def test_host_checks_without_a_device(built):
     """The library refuses bad arguments on the host, before any CUDA call."""
-    from spinnv2_b200 import transformer as T
 
     def call(name, args):
-        return T._function(name)(args, None)
+        return c_function(name)(args, None)
 
     fake = 4096  # never read
-    norm = lambda **c: T._NORM.pack(*{**dict(x=fake, r=0, w=fake, s=0, c=fake, sc=fake, rows=2, width=8, xs=8, rs=0, ss=0, cs=8, eps=0.0, t=1), **c}.values())  # noqa: E731
+    norm = lambda **c: NORM.pack(*{**dict(x=fake, r=0, w=fake, s=0, c=fake, sc=fake, rows=2, width=8, xs=8, rs=0, ss=0, cs=8, eps=0.0, t=1), **c}.values())  # noqa: E731
     for bad in (dict(x=0), dict(w=0), dict(c=0), dict(sc=0), dict(rows=-1), dict(width=0), dict(xs=-1), dict(cs=7), dict(s=fake, ss=4), dict(eps=-1.0), dict(eps=math.nan), dict(width=1 << 25)):
         assert call("spkv2_cuda_rms_norm_i8", norm(**bad)) == -1, bad
     assert call("spkv2_cuda_rms_norm_i8", norm(t=2)) == -43
     assert call("spkv2_cuda_rms_norm_i8", norm(rows=0)) == 0
-    assert T._function("spkv2_cuda_rms_norm_i8")(None, None) == -1
-    lin = lambda **c: T._LINEAR.pack(*{**dict(a=fake, sa=fake, w=fake, sw=fake, b=0, y=fake, m=2, n=2, k=2, as_=2, ws=2, ys=2, t=1, act=0), **c}.values())  # noqa: E731
+    assert c_function("spkv2_cuda_rms_norm_i8")(None, None) == -1
+    lin = lambda **c: LINEAR_ARGS.pack(*{**dict(a=fake, sa=fake, w=fake, sw=fake, b=0, y=fake, m=2, n=2, k=2, as_=2, ws=2, ys=2, t=1, act=0), **c}.values())  # noqa: E731
     for bad in (dict(a=0), dict(sa=0), dict(w=0), dict(sw=0), dict(y=0), dict(m=-1), dict(k=-1), dict(as_=-1), dict(ys=1), dict(act=3), dict(act=-1)):
         assert call("spkv2_cuda_linear_i8", lin(**bad)) == -1, bad
     assert call("spkv2_cuda_linear_i8", lin(k=1 << 17)) == -43 and call("spkv2_cuda_linear_i8", lin(t=9)) == -43
-    assert call("spkv2_cuda_linear_i8", lin(m=0)) == 0 and T._function("spkv2_cuda_linear_i8")(None, None) == -1
+    assert call("spkv2_cuda_linear_i8", lin(m=0)) == 0 and c_function("spkv2_cuda_linear_i8")(None, None) == -1
     base = dict(q=fake, k=fake, v=fake, o=fake, l=0, m=0, b=1, lq=1, lk=1)
     base.update({f"st{i}": 8 for i in range(12)}, ms=0, h=2, hk=1, d=8, t=1, sc=1.0, r=0)
-    cross = lambda **c: T._CROSS.pack(*{**base, **c}.values())  # noqa: E731
+    cross = lambda **c: CROSS.pack(*{**base, **c}.values())  # noqa: E731
     for bad in (dict(q=0), dict(k=0), dict(o=0), dict(b=-1), dict(lk=-1), dict(h=3, hk=2), dict(hk=0), dict(d=0), dict(st4=-1), dict(sc=math.nan), dict(m=fake, ms=-1)):
         assert call("spkv2_cuda_cross_attention", cross(**bad)) == -1, bad
     for bad in (dict(d=257), dict(t=2), dict(lk=1 << 31), dict(lq=1 << 31)):
@@ -540,11 +555,6 @@ def test_host_checks_without_a_device(built):
 
 def test_argument_layout_matches_the_header(built, tmp_path):
     """The packed arguments have the sizes of the C structs."""
-    import subprocess
-    from pathlib import Path
-
-    from spinnv2_b200 import transformer as T
-
     repo = Path(__file__).resolve().parents[1]
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "spkv2_transformer.h"\nint main(void) { printf("%zu %zu %zu %zu %zu", '
@@ -553,10 +563,10 @@ def test_argument_layout_matches_the_header(built, tmp_path):
     exe = tmp_path / "sizes"
     subprocess.run(["gcc", "-std=c99", "-I", str(repo / "include"), str(src), "-o", str(exe)], check=True)
     sizes = [int(s) for s in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-    assert sizes == [T._NORM.size, T._CODES.size, T._CODES.size, T._LINEAR.size, T._CROSS.size]
+    assert sizes == [NORM.size, CODES.size, CODES.size, LINEAR_ARGS.size, CROSS.size]
 
 
-def test_cpu_tensors_are_refused():
+def test_cpu_tensors_are_refused(built):
     from spinnv2_b200 import transformer as T
 
     x = torch.zeros(2, 8)
