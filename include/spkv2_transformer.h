@@ -142,6 +142,13 @@ typedef struct {
 
 int spkv2_cuda_cross_attention(const Spkv2CrossAttention *args, void *stream);
 
+/* Every wait inside the kernels has a limit of about a second; one that runs
+ * out records a role code (2 operand loads, 3 matrix products, 4 results, 7
+ * hand-over) on the device and lets its kernel return, with its outputs
+ * incomplete.  This call waits for the current device's work and returns 0, or
+ * SPKV2_ERR_DEVICE_STATUS with the first such code since the last call. */
+int spkv2_cuda_transformer_status(int *code);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

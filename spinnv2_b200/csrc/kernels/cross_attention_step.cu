@@ -366,4 +366,6 @@ int cross_step(const AttnArgs &a, int32_t dtype, cudaStream_t s) {
   return dtype == SPKV2_DTYPE_FP16 ? launch_type<__half>(a, s) : launch_type<__nv_bfloat16>(a, s);
 }
 
+int cross_step_status(int *code) { return take_status(g_step_status, code); }
+
 }  // namespace spkv2

@@ -510,4 +510,6 @@ int cross_tc(const AttnArgs &a, int32_t dtype, cudaStream_t s) {
   return a.width <= 64 ? launch_tiles<__nv_bfloat16, 64>(a, s) : launch_tiles<__nv_bfloat16, 128>(a, s);
 }
 
+int cross_tc_status(int *code) { return take_status(g_cross_status, code); }
+
 }  // namespace spkv2

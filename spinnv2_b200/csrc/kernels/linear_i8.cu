@@ -586,6 +586,8 @@ int launch_tc(LinearArgs p, cudaStream_t s) {
 
 }  // namespace
 
+int linear_status(int *code) { return take_status(g_linear_status, code); }
+
 }  // namespace spkv2
 
 using namespace spkv2;
@@ -610,4 +612,18 @@ extern "C" int spkv2_cuda_linear_i8(const Spkv2LinearI8 *a, void *stream) {
     linear_simt_kernel<T><<<unsigned(tiles), 256, 0, s>>>(p);
     return cuda_status(cudaGetLastError());
   });
+}
+
+extern "C" int spkv2_cuda_transformer_status(int *code) {
+  if (!code) return -1;
+  *code = 0;
+  int (*const take[])(int *) = {linear_status, cross_tc_status, cross_step_status};
+  int first = 0;
+  for (auto t : take) {
+    int c = 0;
+    if (const int rc = t(&c)) return rc;
+    if (!first) first = c;
+  }
+  *code = first;
+  return first ? SPKV2_ERR_DEVICE_STATUS : 0;
 }

@@ -81,5 +81,22 @@ inline int allow_smem(size_t bytes) {
   return cuda_status(err);
 }
 
+// Reads and clears the status word (a device variable) of a file's kernels on
+// the current device; waits for the device's work.
+template <class Word>
+inline int take_status(Word &word, int *code) {
+  *code = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(code, word, sizeof(int));
+  const int zero = 0;
+  if (err == cudaSuccess && *code) err = cudaMemcpyToSymbol(word, &zero, sizeof(int));
+  return cuda_status(err);
+}
+
 }  // namespace xf
+
+// The status words of the kernels that wait with a limit.
+int linear_status(int *code);
+int cross_tc_status(int *code);
+int cross_step_status(int *code);
+
 }  // namespace spkv2

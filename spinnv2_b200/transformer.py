@@ -90,3 +90,13 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale: float | None
     query without keys is answered with zeros.  scale: 1 / sqrt(width) by default.
     """
     return _ops.cross_attention(q, k, v, lengths, key_mask, scale, out, stream)
+
+
+def check(device=None) -> None:
+    """Waits for the device's work and raises Spkv2Error if a kernel of these calls gave up a bounded wait
+    since the last check (its outputs are then incomplete)."""
+    with torch.cuda.device(device):
+        code = ctypes.c_int(0)
+        rc = load_library().spkv2_cuda_transformer_status(ctypes.byref(code))
+    if rc != 0:
+        raise Spkv2Error(f"wait (code {code.value})", rc, load_library().spkv2_cuda_status_string(rc).decode())

@@ -576,3 +576,14 @@ def test_cpu_tensors_are_refused(built):
         T.quantize_rows_i8([1.0])
 
 
+
+
+@gpu_test
+def test_check_after_calls(gpu):
+    """No wait gave up in the calls before, and the status call says so."""
+    from spinnv2_b200 import transformer as T
+
+    q, k, v = inputs(2, 40, 300, 4, 2, 64, torch.bfloat16)
+    T.cross_attention(q, k, v)
+    T.check()
+    T.check(0)
