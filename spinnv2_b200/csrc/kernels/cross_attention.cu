@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a, int csize, 
   constexpr int CPT = D / 16;  // columns of a thread: tx * CW + 16 * CW * c
   constexpr int CW = CPT < 4 ? CPT : 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  pdl_launch_dependents();
+  pdl_wait();
   const int rank = csize > 1 ? int(cluster_rank()) : 0;
   int t = int(blockIdx.x) / csize;
   const int r0 = t % a.row_tiles * S::rows;
@@ -251,19 +253,7 @@ int launch_simt(AttnArgs a, cudaStream_t s) {
   int csize = 1;
   while (csize < kMaxCluster && blocks * csize * 2 <= 2 * sm_count() && ceil_div(a.keys, kKeys) >= 2 * csize) csize *= 2;
   if (blocks * csize > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  // Without programmatic launch: the kernel reads global memory from its start.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks * csize));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = sizeof(S);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(csize);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = csize > 1 ? 1 : 0;
-  return cuda_status(cudaLaunchKernelEx(&cfg, cross_simt_kernel<T, D, R>, a, csize, vec));
+  return cuda_status(launch_kernel(cross_simt_kernel<T, D, R>, unsigned(blocks * csize), 256u, sizeof(S), s, csize, a, csize, vec));
 }
 
 // Sixteen rows a tile where they are all there are, else 64.

@@ -34,6 +34,8 @@ constexpr int kST = 64, kSK = 64, kSPitch = kSK + 4;
 
 template <class T>
 __global__ void __launch_bounds__(256) linear_simt_kernel(LinearArgs p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ __align__(16) int8_t sa[kST][kSPitch];
   __shared__ __align__(16) int8_t sw[kST][kSPitch];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -609,8 +611,7 @@ extern "C" int spkv2_cuda_linear_i8(const Spkv2LinearI8 *a, void *stream) {
     return by_type(a->dtype, [&](auto t) { return launch_tc<decltype(t)>(p, s); });
   return by_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    linear_simt_kernel<T><<<unsigned(tiles), 256, 0, s>>>(p);
-    return cuda_status(cudaGetLastError());
+    return cuda_status(launch_kernel(linear_simt_kernel<T>, unsigned(tiles), 256u, 0, s, 1, p));
   });
 }
 

@@ -10,6 +10,7 @@
 // Quantising without the norm is the same with r = 0, w = 1 and no factor.
 //
 // The maximum keeps a NaN, so it says by itself whether the row is finite.
+#include "tcgen05.cuh"
 #include "transformer.cuh"
 
 namespace spkv2 {
@@ -17,6 +18,7 @@ namespace spkv2 {
 namespace {
 
 using namespace xf;
+using namespace tc;
 
 constexpr int64_t kMaxWidth = int64_t(1) << 24, kMostWidth = 16384;  // of a call; of rows kept in registers
 constexpr int kPerThread = 16;  // elements; with 8 the synchronisation costs more (40000 x 512 in bf16: 29 us, with 16 24 us)
@@ -139,6 +141,8 @@ __host__ __device__ __forceinline__ int stage_floats(int width, int u) { return 
 template <class T, bool NORM, bool STAGED>
 __global__ void __launch_bounds__(1024)
     row_codes_kernel(RowArgs p, int tpr, int rpb, bool vec_codes, bool vec_weight) {
+  pdl_launch_dependents();
+  pdl_wait();
   constexpr int U = 16 / sizeof(T), N = kPerThread / U;
   extern __shared__ __align__(16) float staged[];
   __shared__ float s_sum[32], s_max[32];
@@ -317,6 +321,8 @@ __global__ void __launch_bounds__(1024)
 // second pass, as it may take x's or the residual's place.
 template <class T, bool NORM>
 __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float s_sum[32];
   __shared__ float s_max[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
@@ -368,6 +374,8 @@ template <class T, int VW>
 __global__ void __launch_bounds__(256)
     row_values_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, uint32_t chunks,
                       FastDiv per_row, int64_t codes_stride, int64_t y_stride) {
+  pdl_launch_dependents();
+  pdl_wait();
   for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < chunks; i += gridDim.x * 256u) {
     const uint32_t row = per_row.div(i), c = (i - row * per_row.d) * VW;
     const float s = __ldg(scale + row);
@@ -391,6 +399,8 @@ template <class T>
 __global__ void __launch_bounds__(256)
     row_values_shifted_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, int width,
                               uint32_t chunks, FastDiv per_row, int64_t codes_stride, int64_t y_stride) {
+  pdl_launch_dependents();
+  pdl_wait();
   constexpr int U = 16 / sizeof(T);
   for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < chunks; i += gridDim.x * 256u) {
     const uint32_t row = per_row.div(i), k = i - row * per_row.d;
@@ -427,8 +437,8 @@ int launch_row(const RowArgs &a, bool vec_codes, cudaStream_t s) {
   const size_t smem = STAGED ? size_t(rpb) * stage_floats(int(a.width), U) * 4 : 0;
   if (STAGED)
     if (const int rc = allow_smem<kern>(stage_floats(kMostWidth, U) * 4)) return rc;
-  kern<<<unsigned(ceil_div(a.rows, rpb)), tpr * rpb, smem, s>>>(a, tpr, rpb, vec_codes, aligned16(a.weight));
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_kernel(kern, unsigned(ceil_div(a.rows, rpb)), unsigned(tpr * rpb), smem, s, 1, a, tpr, rpb, vec_codes,
+                                   aligned16(a.weight)));
 }
 
 // The most elements (a power of two up to `most`) that rows can be accessed by:
@@ -445,8 +455,7 @@ int launch_rows(const RowArgs &a, int32_t dtype, cudaStream_t s) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     if (a.width > kMostWidth) {
-      wide_codes_kernel<T, NORM><<<unsigned(a.rows), 1024, 0, s>>>(a);
-      return cuda_status(cudaGetLastError());
+      return cuda_status(launch_kernel(wide_codes_kernel<T, NORM>, unsigned(a.rows), 1024u, 0, s, 1, a));
     }
     constexpr int U = 16 / sizeof(T);
     auto apart = [&](const void *base, int64_t stride) { return !aligned16(base) || (a.rows > 1 && stride % U != 0); };
@@ -464,9 +473,8 @@ int launch_values(const Spkv2DequantizeRowsI8 *a, cudaStream_t s) {
   if (chunks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
   // Several chunks a thread once all SMs are full (eight blocks each).
   const unsigned grid = unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64));
-  row_values_kernel<T, VW><<<grid, 256, 0, s>>>(a->codes, a->scale, static_cast<T *>(a->y), uint32_t(chunks),
-                                                FastDiv(uint32_t(per_row)), a->codes_stride, a->y_stride);
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_kernel(row_values_kernel<T, VW>, grid, 256u, 0, s, 1, a->codes, a->scale, static_cast<T *>(a->y),
+                                   uint32_t(chunks), FastDiv(uint32_t(per_row)), a->codes_stride, a->y_stride));
 }
 
 bool bad_extent(int64_t rows, int64_t width) { return rows < 0 || rows > INT32_MAX || width < 1 || width > kMaxWidth; }
@@ -516,10 +524,10 @@ extern "C" int spkv2_cuda_dequantize_rows_i8(const Spkv2DequantizeRowsI8 *a, voi
     if (std::min(vw, vy) < 16 / int(size)) {
       const int64_t per_row = 1 + ceil_div(a->width, 16 / size), chunks = per_row * a->rows;
       if (chunks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-      row_values_shifted_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64)), 256, 0, s>>>(
-          a->codes, a->scale, static_cast<T *>(a->y), int(a->width), uint32_t(chunks), FastDiv(uint32_t(per_row)),
-          a->codes_stride, a->y_stride);
-      return cuda_status(cudaGetLastError());
+      const unsigned grid = unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64));
+      return cuda_status(launch_kernel(row_values_shifted_kernel<T>, grid, 256u, 0, s, 1, a->codes, a->scale,
+                                       static_cast<T *>(a->y), int(a->width), uint32_t(chunks), FastDiv(uint32_t(per_row)),
+                                       a->codes_stride, a->y_stride));
     }
     if (vw == 16) return launch_values<T, 16>(a, s);
     if (size == 2 || vw == 8) return launch_values<T, 8>(a, s);
