@@ -75,17 +75,13 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a, int csize, 
   const int keys = entry_keys(a, b), tiles = (keys + kKeys - 1) / kKeys;
   const int tile0 = int(int64_t(tiles) * rank / csize), tile1 = int(int64_t(tiles) * (rank + 1) / csize);
   auto out_row = [&](int row) {
-    const int qi = row / a.group, h = hk * a.group + row % a.group;
-    return static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+    return static_cast<T *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row);
   };
 
   for (int e = tid; e < S::rows * D; e += 256) {
     const int r = e / D, c = e % D, row = r0 + r;
     float val = 0.0f;
-    if (row < a.rows && c < a.width) {
-      const int qi = row / a.group, h = hk * a.group + row % a.group;
-      val = to_f32(q[qi * a.qs[1] + h * a.qs[2] + c]);
-    }
+    if (row < a.rows && c < a.width) val = to_f32(q[row_offset(a, a.qs, hk, row) + c]);
     sm.q[r][c] = val;
   }
   float o[R][CPT] = {}, m[R], l[R] = {};
@@ -292,6 +288,7 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   a.batch = int(x->batch), a.queries = int(x->queries), a.keys = int(x->keys);
   a.kv_heads = x->kv_heads, a.group = group, a.width = x->width;
   a.rows = a.queries * group;
+  a.group_div = FastDiv(uint32_t(group));
   a.scale_log2 = x->scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (cross_tc_serves(a, x->dtype)) return a.rows <= 32 ? cross_step(a, x->dtype, s) : cross_tc(a, x->dtype, s);

@@ -20,7 +20,15 @@ struct AttnArgs {
   int rows;        // queries * group
   int row_tiles;   // per (batch, key head)
   float scale_log2;
+  FastDiv group_div;
 };
+
+// Element offset of a row (query * group + head in the group) of q or out, from the
+// entry's start.
+__device__ __forceinline__ int64_t row_offset(const AttnArgs &p, const int64_t (&st)[3], int hk, int row) {
+  const uint32_t qi = p.group_div.div(uint32_t(row));
+  return int64_t(qi) * st[1] + (int64_t(hk) * p.group + (uint32_t(row) - qi * uint32_t(p.group))) * st[2];
+}
 
 __device__ __forceinline__ int entry_keys(const AttnArgs &p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;

@@ -31,10 +31,13 @@ struct Step {
   static constexpr int half_bytes = kChunk * 128;            // 64 columns of a chunk
   static constexpr int stage_bytes = 2 * halves * half_bytes;  // K and V
   static constexpr int stages = D == 128 ? 3 : 6;
-  static constexpr int ring_bytes = stages * stage_bytes;  // a warp's
-  static constexpr int part_floats = MT * 16 * D;          // a warp's O at the end, over its ring
-  static constexpr size_t smem = size_t(kWarps) * ring_bytes + 1024;
-  static_assert(part_floats * 4 <= ring_bytes, "a warp's sums reuse its ring");
+  static constexpr int part_bytes = MT * 16 * D * 4;  // a warp's O at the end, over its ring
+  // A warp's ring, for a warp with `chunks` chunks: short ones leave room for more
+  // CTAs on the SM.
+  static constexpr int ring_bytes(int chunks) {
+    const int ring = (chunks < stages ? chunks : stages) * stage_bytes;
+    return ring < part_bytes ? part_bytes : ring;
+  }
 };
 
 __device__ int g_step_status;  // role code of the last bounded wait that gave up
@@ -88,9 +91,9 @@ struct Mma<__nv_bfloat16> {
 };
 
 template <class T, int D, int MT>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, MT == 1 ? (D == 64 ? 4 : 3) : 2)
     cross_step_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a,
-                      int k_heads_step, int k_batch_step, int v_heads_step, int v_batch_step, int csize) {
+                      int k_heads_step, int k_batch_step, int v_heads_step, int v_batch_step, int csize, int ring_bytes) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using S = Step<D, MT>;
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int rank = csize > 1 ? int(cluster_rank()) : 0;
   const int item = int(blockIdx.x) / csize;
   const int hk = item % a.kv_heads, b = item / a.kv_heads;
-  uint8_t *ring = smem + warp * S::ring_bytes;
+  uint8_t *ring = smem + warp * ring_bytes;
   if (lane == 0)
     for (int s = 0; s < S::stages; ++s) mbar_init(&full_bar[warp][s], 1);
   if (tid == 0) abort_flag = 0;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int first = int(int64_t(chunks) * rank / csize) + warp;
   const int last = int(int64_t(chunks) * (rank + 1) / csize);  // this warp's chunks: first, first + 4, .. below last
   const int mine = last > first ? (last - first + kWarps - 1) / kWarps : 0;
-  auto load = [&](int n) {  // lane 0: this warp's n-th chunk
+  auto load = [&](int n) {  // one lane: this warp's n-th chunk
     const int slot = n % S::stages, j0 = (first + n * kWarps) * kChunk;
     uint8_t *st = ring + slot * S::stage_bytes;
     mbar_arrive_expect_tx(&full_bar[warp][slot], S::stage_bytes);
@@ -129,8 +132,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                   &full_bar[warp][slot]);
     }
   };
-  if (lane == 0)
+  if (elect_one())
     for (int n = 0; n < S::stages && n < mine; ++n) load(n);
+  __syncwarp();
 
   // Fragments: a lane holds rows g and g + 8 of a 16-row tile, columns 2 t,
   // 2 t + 1 (and + 8) of each 16.
@@ -143,8 +147,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int row = mt * 16 + half * 8 + g;
-        const int qi = row / a.group, h = hk * a.group + row % a.group;
-        const T *src = q + qi * a.qs[1] + h * a.qs[2];
+        const T *src = q + row_offset(a, a.qs, hk, row);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -258,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     if (bits != 0xffffu) fence_proxy_async();  // the zeros above precede the next load into this slot
     __syncwarp();
-    if (lane == 0 && n + S::stages < mine) load(n + S::stages);
+    if (n + S::stages < mine && elect_one()) load(n + S::stages);
   }
   if (n < mine && lane == 0) {  // giving up: what was issued lands (bounded) before shared memory goes away
     for (int k = n; k < n + S::stages && k < mine; ++k) {
@@ -298,14 +301,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int w = 0; w < kWarps; ++w) {
       const float f = weight(s_m[w][r], top);
       // A warp without keys has sums of 0; one whose maximum is not finite has NaN.
-      acc += reinterpret_cast<float *>(smem + w * S::ring_bytes)[e] * f;
+      acc += reinterpret_cast<float *>(smem + w * ring_bytes)[e] * f;
       sum += s_l[w][r] * f;
     }
     if (csize == 1) {
       const int c = e % D;
       if (c < a.width && !abort_flag) {
-        const int qi = r / a.group, h = hk * a.group + r % a.group;
-        static_cast<T *>(a.out)[b * a.os[0] + qi * a.os[1] + h * a.os[2] + c] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+        static_cast<T *>(a.out)[b * a.os[0] + row_offset(a, a.os, hk, r) + c] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
       }
     } else {
       reinterpret_cast<float *>(smem)[e] = acc;
@@ -329,8 +331,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         sum += __uint_as_float(ld_cluster(map_rank(&c_l[r], k))) * f;
       }
       if (c < a.width && !abort_flag) {
-        const int qi = r / a.group, h = hk * a.group + r % a.group;
-        static_cast<T *>(a.out)[b * a.os[0] + qi * a.os[1] + h * a.os[2] + c] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+        static_cast<T *>(a.out)[b * a.os[0] + row_offset(a, a.os, hk, r) + c] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
       }
     }
     __syncwarp();
@@ -341,17 +342,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <class T, int D, int MT>
 int launch(const AttnArgs &a, cudaStream_t s) {
   using S = Step<D, MT>;
-  if (const int rc = allow_smem<cross_step_kernel<T, D, MT>>(S::smem)) return rc;
+  if (const int rc = allow_smem<cross_step_kernel<T, D, MT>>(size_t(kWarps) * S::ring_bytes(S::stages) + 1024)) return rc;
   KvMap k, v;
   if (!encode_kv(&k, a, a.k, a.ks, kChunk) || !encode_kv(&v, a, a.v, a.vs, kChunk)) return SPKV2_ERR_CUDA;
-  // Divide the keys while a CTA keeps 16 chunks (4 a warp), up to eight CTAs an
-  // SM: entries differ in length, and more, shorter pieces even that out.
   const int64_t items = int64_t(a.batch) * a.kv_heads;
+  auto warp_chunks = [&](int c) { return int(ceil_div(ceil_div(a.keys, kChunk), int64_t(c) * kWarps)); };
+  // Divide the keys while the CTAs are at most two an SM and a warp keeps more
+  // than two chunks.  More CTAs than that only queue, and a cluster costs its CTAs
+  // a start together and two barriers: 512 entries and heads of 500 keys (width
+  // 64) take 21 us undivided, 24 by two, 27 by four; 16 of 4096 keys 34 us, 19,
+  // 12, and 9 by eight.
   int csize = 1;
-  while (csize < 8 && a.keys >= 2 * csize * 16 * kChunk && items * csize < 8 * sm_count()) csize *= 2;
+  while (csize < 8 && items * csize <= sm_count() && warp_chunks(csize) > 2) csize *= 2;
   if (items * csize > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  return cuda_status(launch_kernel(cross_step_kernel<T, D, MT>, unsigned(items * csize), kThreads, S::smem, s, csize, k.map,
-                                   v.map, a, k.heads_step, k.batch_step, v.heads_step, v.batch_step, csize));
+  const int ring = S::ring_bytes(warp_chunks(csize));
+  return cuda_status(launch_kernel(cross_step_kernel<T, D, MT>, unsigned(items * csize), kThreads, size_t(kWarps) * ring + 1024, s,
+                                   csize, k.map, v.map, a, k.heads_step, k.batch_step, v.heads_step, v.batch_step, csize, ring));
 }
 
 template <class T>

@@ -171,8 +171,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
 
   float *part = reinterpret_cast<float *>(smem);  // O for the cluster's join, [tile][column][row], over Q, K and V
   auto out_row = [&](int row) {
-    const int qi = row / a.group, h = hk * a.group + row % a.group;
-    return static_cast<T *>(a.out) + b * a.os[0] + qi * a.os[1] + h * a.os[2];
+    return static_cast<T *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row);
   };
 
   if (warp < SOFT) {
@@ -184,15 +183,22 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
       const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
       constexpr int CH = D / 8, RPI = 32 / CH;  // chunks of a row, rows of an iteration
       const int c = lane % CH;
-#pragma unroll 4
-      for (int k = 0; k < 32 / RPI; ++k) {
-        const int rr = quarter * 32 + k * RPI + lane / CH, row = r0 + i * kTile + rr;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < a.rows && c * 8 < a.width) {
-          const int qi = row / a.group, h = hk * a.group + row % a.group;
-          v = __ldg(reinterpret_cast<const uint4 *>(q + qi * a.qs[1] + h * a.qs[2] + c * 8));
+      constexpr int B = 8;  // loads in flight
+#pragma unroll
+      for (int k0 = 0; k0 < 32 / RPI; k0 += B) {
+        uint4 v[B];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const int row = r0 + i * kTile + quarter * 32 + (k0 + k) * RPI + lane / CH;
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (row < a.rows && c * 8 < a.width)
+            v[k] = __ldg(reinterpret_cast<const uint4 *>(q + row_offset(a, a.qs, hk, row) + c * 8));
         }
-        *reinterpret_cast<uint4 *>(smem + i * S::tile_bytes + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const int rr = quarter * 32 + (k0 + k) * RPI + lane / CH;
+          *reinterpret_cast<uint4 *>(smem + i * S::tile_bytes + (c >> 3) * kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[k];
+        }
       }
       fence_proxy_async();
       __syncwarp();
