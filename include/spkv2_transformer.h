@@ -18,7 +18,8 @@
  * Conventions of all of them:
  *   - Every pointer is device memory of the current device.  Strides count
  *     elements; the last dimension is contiguous.  A pointer or stride that
- *     is not a multiple of 16 bytes is served, by a slower kernel.
+ *     is not a multiple of 16 bytes is served, by a slower kernel; a pointer
+ *     that is not a multiple of its element's size is a bad argument.
  *   - The call checks its arguments on the host, launches one kernel on
  *     `stream` (a cudaStream_t; NULL = legacy default stream) and returns.
  *     It allocates nothing, keeps nothing and can be captured into a graph.
@@ -87,7 +88,7 @@ typedef struct {
 
 int spkv2_cuda_quantize_rows_i8(const Spkv2QuantizeRowsI8 *args, void *stream);
 
-/* y = codes * scale[row]. */
+/* y = codes * scale[row]; up to 2^33 elements. */
 typedef struct {
     const int8_t *codes; /* [rows, width] */
     const float *scale;  /* [rows] */

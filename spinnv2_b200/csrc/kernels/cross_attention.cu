@@ -53,6 +53,12 @@ __device__ __forceinline__ float4 load4(const T *p) {
   return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
 }
 
+// The first `left` of four elements, one by one; zeros behind them.
+template <class T>
+__device__ __forceinline__ float4 load_up_to4(const T *p, int left) {
+  return make_float4(to_f32(p[0]), left > 1 ? to_f32(p[1]) : 0.0f, left > 2 ? to_f32(p[2]) : 0.0f, left > 3 ? to_f32(p[3]) : 0.0f);
+}
+
 template <class T, int D, int R>
 __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a, int csize, bool vec) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -78,43 +84,77 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(AttnArgs a, int csize, 
     return static_cast<T *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row);
   };
 
-  for (int e = tid; e < S::rows * D; e += 256) {
+  // A tile's keys and values, four elements of a row a piece: into registers, and
+  // from there into shared memory once the last tile's readers are done.  Up to 64
+  // columns the registers last to load a tile while the one before is computed.
+  constexpr bool AHEAD = D <= 64;
+  constexpr int PIECES = kKeys * D / 4 / 256, HELD = AHEAD ? PIECES : 1;
+  float4 kr[HELD], vr[HELD];
+  bool counts[HELD];
+  auto piece = [&](int n, int &r, int &c) {
+    const int e = (tid + n * 256) * 4;
+    r = e / D, c = e % D;
+  };
+  auto fetch = [&](int tile, int n, float4 &kf, float4 &vf, bool &in) {
+    int r, c;
+    piece(n, r, c);
+    const int j = tile * kKeys + r;
+    in = j < keys && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
+    kf = vf = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!in || c >= a.width) return;
+    const T *kp = k + j * a.ks[1] + c, *vp = v + j * a.vs[1] + c;
+    if (vec) {
+      kf = load4(kp);
+      vf = load4(vp);
+    } else {
+      kf = load_up_to4(kp, a.width - c);
+      vf = load_up_to4(vp, a.width - c);
+    }
+  };
+  auto put = [&](int n, const float4 &kf, const float4 &vf, bool in) {
+    int r, c;
+    piece(n, r, c);
+    *reinterpret_cast<float4 *>(&sm.k[r][c]) = kf;
+    *reinterpret_cast<float4 *>(&sm.v[r][c]) = vf;
+    if (c == 0) sm.valid[r] = in;
+  };
+  if (AHEAD && tile0 < tile1) {
+#pragma unroll
+    for (int n = 0; n < HELD; ++n) fetch(tile0, n, kr[n], vr[n], counts[n]);
+  }
+#pragma unroll 4
+  for (int e = tid * 4; e < S::rows * D; e += 1024) {
     const int r = e / D, c = e % D, row = r0 + r;
-    float val = 0.0f;
-    if (row < a.rows && c < a.width) val = to_f32(q[row_offset(a, a.qs, hk, row) + c]);
-    sm.q[r][c] = val;
+    float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (row < a.rows && c < a.width) {
+      const T *qp = q + row_offset(a, a.qs, hk, row) + c;
+      val = vec ? load4(qp) : load_up_to4(qp, a.width - c);
+    }
+    *reinterpret_cast<float4 *>(&sm.q[r][c]) = val;
   }
   float o[R][CPT] = {}, m[R], l[R] = {};
 #pragma unroll
   for (int i = 0; i < R; ++i) m[i] = -INFINITY;
 
   for (int tile = tile0; tile < tile1; ++tile) {
-    const int j0 = tile * kKeys;
     __syncthreads();  // the last tile's readers are done
-    if (tid < kKeys) {
-      const int j = j0 + tid;
-      sm.valid[tid] = j < keys && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
-    }
-    __syncthreads();
-    if (vec) {
-#pragma unroll 4
-      for (int e = tid * 4; e < kKeys * D; e += 1024) {
-        const int r = e / D, c = e % D;
-        const bool in = sm.valid[r] && c < a.width;
-        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        *reinterpret_cast<float4 *>(&sm.k[r][c]) = in ? load4(k + (j0 + r) * a.ks[1] + c) : zero;
-        *reinterpret_cast<float4 *>(&sm.v[r][c]) = in ? load4(v + (j0 + r) * a.vs[1] + c) : zero;
-      }
+    if (AHEAD) {
+#pragma unroll
+      for (int n = 0; n < HELD; ++n) put(n, kr[n], vr[n], counts[n]);
     } else {
 #pragma unroll 4
-      for (int e = tid; e < kKeys * D; e += 256) {
-        const int r = e / D, c = e % D;
-        const bool in = sm.valid[r] && c < a.width;
-        sm.k[r][c] = in ? to_f32(k[(j0 + r) * a.ks[1] + c]) : 0.0f;
-        sm.v[r][c] = in ? to_f32(v[(j0 + r) * a.vs[1] + c]) : 0.0f;
+      for (int n = 0; n < PIECES; ++n) {
+        float4 kf, vf;
+        bool in;
+        fetch(tile, n, kf, vf, in);
+        put(n, kf, vf, in);
       }
     }
     __syncthreads();
+    if (AHEAD && tile + 1 < tile1) {
+#pragma unroll
+      for (int n = 0; n < HELD; ++n) fetch(tile + 1, n, kr[n], vr[n], counts[n]);
+    }
     float s[R][4] = {};
 #pragma unroll 4
     for (int c = 0; c < D; c += 4) {
@@ -244,7 +284,7 @@ int launch_simt(AttnArgs a, cudaStream_t s) {
   auto fours = [](const void *base, const int64_t (&st)[3]) {
     return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
   };
-  const bool vec = a.width % 4 == 0 && fours(a.k, a.ks) && fours(a.v, a.vs);
+  const bool vec = a.width % 4 == 0 && fours(a.q, a.qs) && fours(a.k, a.ks) && fours(a.v, a.vs);
   // Divide the keys while a CTA keeps a tile and the CTAs are fewer than two an SM.
   int csize = 1;
   while (csize < kMaxCluster && blocks * csize * 2 <= 2 * sm_count() && ceil_div(a.keys, kKeys) >= 2 * csize) csize *= 2;
@@ -279,6 +319,7 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   if (!elem_bytes(x->dtype) || x->width > 256 || x->batch > INT32_MAX || x->keys > INT32_MAX - 1024 ||
       x->queries > (INT32_MAX - 1024) / group)
     return SPKV2_ERR_UNSUPPORTED;
+  if (!on_bytes(elem_bytes(x->dtype), x->q, x->k, x->v, x->out) || !on_bytes(4, x->lengths)) return -1;
   AttnArgs a = {};
   a.q = x->q, a.k = x->k, a.v = x->v, a.out = x->out, a.lengths = x->lengths, a.key_mask = x->key_mask;
   for (int i = 0; i < 3; ++i) {

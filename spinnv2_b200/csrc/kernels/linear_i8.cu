@@ -13,7 +13,8 @@ namespace {
 using namespace xf;
 using namespace tc;
 
-constexpr int64_t kMaxK = 131071;  // 128 * 128 * k stays below 2^31
+constexpr int64_t kMaxK = 131071;              // 128 * 128 * k stays below 2^31
+constexpr int64_t kMostRows = INT32_MAX - 1024;  // tile coordinates stay 32-bit numbers
 
 struct LinearArgs {
   const int8_t *a, *w;
@@ -601,7 +602,8 @@ extern "C" int spkv2_cuda_linear_i8(const Spkv2LinearI8 *a, void *stream) {
   if (!a->y || !a->a_scale || !a->w_scale || (a->k > 0 && (!a->a || !a->w))) return -1;
   if (a->a_stride < 0 || a->w_stride < 0 || overlaps(a->y_stride, a->m, a->n)) return -1;
   if (a->activation < SPKV2_CUDA_ACT_NONE || a->activation > SPKV2_CUDA_ACT_SILU) return -1;
-  if (!elem_bytes(a->dtype) || a->k > kMaxK || a->m > INT32_MAX || a->n > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  if (!elem_bytes(a->dtype) || a->k > kMaxK || a->m > kMostRows || a->n > kMostRows) return SPKV2_ERR_UNSUPPORTED;
+  if (!on_bytes(elem_bytes(a->dtype), a->y) || !on_bytes(4, a->a_scale, a->w_scale, a->bias)) return -1;
   const LinearArgs p = {a->a, a->w, a->a_scale, a->w_scale, a->bias, a->y, a->m, a->n, a->a_stride, a->w_stride,
                         a->y_stride, int(a->k), a->activation};
   const int64_t tiles = ceil_div(a->m, kST) * ceil_div(a->n, kST);

@@ -494,6 +494,7 @@ extern "C" int spkv2_cuda_rms_norm_i8(const Spkv2RmsNormI8 *a, void *stream) {
       (a->sum && overlaps(a->sum_stride, a->rows, a->width)))
     return -1;
   if (!elem_bytes(a->dtype)) return SPKV2_ERR_UNSUPPORTED;
+  if (!on_bytes(elem_bytes(a->dtype), a->x, a->residual, a->weight, a->sum) || !on_bytes(4, a->scale)) return -1;
   RowArgs p = {a->x,     a->residual, a->weight,   a->sum,      a->codes,           a->scale,      a->rows,
                a->width, a->x_stride, a->residual_stride, a->sum_stride, a->codes_stride, a->eps};
   return launch_rows<true>(p, a->dtype, static_cast<cudaStream_t>(stream));
@@ -504,6 +505,7 @@ extern "C" int spkv2_cuda_quantize_rows_i8(const Spkv2QuantizeRowsI8 *a, void *s
   if (a->rows == 0) return 0;
   if (!a->x || !a->codes || !a->scale || a->x_stride < 0 || overlaps(a->codes_stride, a->rows, a->width)) return -1;
   if (!elem_bytes(a->dtype)) return SPKV2_ERR_UNSUPPORTED;
+  if (!on_bytes(elem_bytes(a->dtype), a->x) || !on_bytes(4, a->scale)) return -1;
   RowArgs p = {a->x, nullptr, nullptr, nullptr, a->codes, a->scale, a->rows, a->width, a->x_stride, 0, 0,
                a->codes_stride, 0.0f};
   return launch_rows<false>(p, a->dtype, static_cast<cudaStream_t>(stream));
@@ -513,6 +515,8 @@ extern "C" int spkv2_cuda_dequantize_rows_i8(const Spkv2DequantizeRowsI8 *a, voi
   if (!a || bad_extent(a->rows, a->width)) return -1;
   if (a->rows == 0) return 0;
   if (!a->codes || !a->scale || !a->y || a->codes_stride < 0 || overlaps(a->y_stride, a->rows, a->width)) return -1;
+  if (!elem_bytes(a->dtype)) return SPKV2_ERR_UNSUPPORTED;
+  if (!on_bytes(elem_bytes(a->dtype), a->y) || !on_bytes(4, a->scale)) return -1;
   return by_type(a->dtype, [&](auto t) {
     using T = decltype(t);
     // Stores of 16 bytes at most: y's alignment beyond them does not matter.

@@ -45,6 +45,12 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // one row for all).
 inline bool overlaps(int64_t stride, int64_t rows, int64_t width) { return rows > 1 ? stride < width : stride < 0; }
 
+// Whether every pointer given (NULL counts as given) is a multiple of `bytes`.
+template <class... P>
+inline bool on_bytes(uintptr_t bytes, const P *...p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0;
+}
+
 // Calls fn(T{}) for the element type of `dtype`, which the caller has checked.
 template <class F>
 inline int by_type(int32_t dtype, F &&fn) {

@@ -533,20 +533,23 @@ def test_host_checks_without_a_device(built):
 
     fake = 4096  # never read
     norm = lambda **c: NORM.pack(*{**dict(x=fake, r=0, w=fake, s=0, c=fake, sc=fake, rows=2, width=8, xs=8, rs=0, ss=0, cs=8, eps=0.0, t=1), **c}.values())  # noqa: E731
-    for bad in (dict(x=0), dict(w=0), dict(c=0), dict(sc=0), dict(rows=-1), dict(width=0), dict(xs=-1), dict(cs=7), dict(s=fake, ss=4), dict(eps=-1.0), dict(eps=math.nan), dict(width=1 << 25)):
+    for bad in (dict(x=0), dict(w=0), dict(c=0), dict(sc=0), dict(rows=-1), dict(width=0), dict(xs=-1), dict(cs=7), dict(s=fake, ss=4), dict(eps=-1.0), dict(eps=math.nan), dict(width=1 << 25),
+                dict(x=fake + 2), dict(s=fake + 1, ss=8), dict(sc=fake + 2)):
         assert call("spkv2_cuda_rms_norm_i8", norm(**bad)) == -1, bad
     assert call("spkv2_cuda_rms_norm_i8", norm(t=2)) == -43
     assert call("spkv2_cuda_rms_norm_i8", norm(rows=0)) == 0
     assert c_function("spkv2_cuda_rms_norm_i8")(None, None) == -1
     lin = lambda **c: LINEAR_ARGS.pack(*{**dict(a=fake, sa=fake, w=fake, sw=fake, b=0, y=fake, m=2, n=2, k=2, as_=2, ws=2, ys=2, t=1, act=0), **c}.values())  # noqa: E731
-    for bad in (dict(a=0), dict(sa=0), dict(w=0), dict(sw=0), dict(y=0), dict(m=-1), dict(k=-1), dict(as_=-1), dict(ys=1), dict(act=3), dict(act=-1)):
+    for bad in (dict(a=0), dict(sa=0), dict(w=0), dict(sw=0), dict(y=0), dict(m=-1), dict(k=-1), dict(as_=-1), dict(ys=1), dict(act=3), dict(act=-1),
+                dict(y=fake + 2), dict(sa=fake + 1), dict(b=fake + 2)):
         assert call("spkv2_cuda_linear_i8", lin(**bad)) == -1, bad
     assert call("spkv2_cuda_linear_i8", lin(k=1 << 17)) == -43 and call("spkv2_cuda_linear_i8", lin(t=9)) == -43
     assert call("spkv2_cuda_linear_i8", lin(m=0)) == 0 and c_function("spkv2_cuda_linear_i8")(None, None) == -1
     base = dict(q=fake, k=fake, v=fake, o=fake, l=0, m=0, b=1, lq=1, lk=1)
     base.update({f"st{i}": 8 for i in range(12)}, ms=0, h=2, hk=1, d=8, t=1, sc=1.0, r=0)
     cross = lambda **c: CROSS.pack(*{**base, **c}.values())  # noqa: E731
-    for bad in (dict(q=0), dict(k=0), dict(o=0), dict(b=-1), dict(lk=-1), dict(h=3, hk=2), dict(hk=0), dict(d=0), dict(st4=-1), dict(sc=math.nan), dict(m=fake, ms=-1)):
+    for bad in (dict(q=0), dict(k=0), dict(o=0), dict(b=-1), dict(lk=-1), dict(h=3, hk=2), dict(hk=0), dict(d=0), dict(st4=-1), dict(sc=math.nan), dict(m=fake, ms=-1),
+                dict(q=fake + 2), dict(l=fake + 2)):
         assert call("spkv2_cuda_cross_attention", cross(**bad)) == -1, bad
     for bad in (dict(d=257), dict(t=2), dict(lk=1 << 31), dict(lq=1 << 31)):
         assert call("spkv2_cuda_cross_attention", cross(**bad)) == -43, bad
