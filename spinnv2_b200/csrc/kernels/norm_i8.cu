@@ -201,6 +201,10 @@ __global__ void __launch_bounds__(1024)
   }
   float v[N][U];
   if (STAGED) {
+    // Places of a unit's elements: element head + k U + e lies at k (U + 1) + place[e].
+    int place[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) place[e] = stage_at(head + e, U);
     if (real) {
       for (int c = t; c < head + width - tail; c += tpr) {
         const int e = c < head ? c : c - head + tail;
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(1024)
           for (int e = 0; e < U; ++e) s[e] += add[e];
         }
 #pragma unroll
-        for (int e = 0; e < U; ++e) mine[stage_at(head + k * U + e, U)] = s[e];
+        for (int e = 0; e < U; ++e) mine[k * (U + 1) + place[e]] = s[e];
         if (NORM && p.sum) *reinterpret_cast<uint4 *>(sum + head + k * U) = contract(s, T{});
       }
       if (t < (width + U - 1) / U * U - width) mine[stage_at(width + t, U)] = 0.0f;
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(1024)
     for (int i = 0; i < N; ++i) {
       const int c = (t + i * tpr) * U;
 #pragma unroll
-      for (int e = 0; e < U; ++e) v[i][e] = real && c < width ? mine[stage_at(c + e, U)] : 0.0f;
+      for (int e = 0; e < U; ++e) v[i][e] = real && c < width ? mine[(t + i * tpr) * (U + 1) + e] : 0.0f;
     }
   } else {
 #pragma unroll
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(256)
 template <class T>
 __global__ void __launch_bounds__(256)
     row_values_shifted_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, int width,
-                              uint32_t chunks, FastDiv per_row, int64_t codes_stride, int64_t y_stride) {
+                              uint32_t chunks, FastDiv per_row, int64_t codes_stride, int64_t y_stride, bool vec_codes) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int U = 16 / sizeof(T);
@@ -412,8 +416,19 @@ __global__ void __launch_bounds__(256)
     const float s = __ldg(scale + row);
     if (k > 0 && c + U <= width) {
       Vec<T, U> o;
+      // The codes from aligned words, where all of them lie inside the row.
+      const int w0 = c & ~3, shift = (c & 3) * 8;
+      if (vec_codes && w0 + U + 4 <= width) {
+        uint32_t w[U / 4 + 1];
 #pragma unroll
-      for (int e = 0; e < U; ++e) o.v[e] = from_f32<T>(float(from[c + e]) * s);
+        for (int i = 0; i <= U / 4; ++i) w[i] = *reinterpret_cast<const uint32_t *>(from + w0 + 4 * i);
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+          o.v[e] = from_f32<T>(float(int8_t(__funnelshift_r(w[e / 4], w[e / 4 + 1], shift) >> (8 * (e & 3)))) * s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < U; ++e) o.v[e] = from_f32<T>(float(from[c + e]) * s);
+      }
       *reinterpret_cast<Vec<T, U> *>(to + c) = o;
     } else {
       for (int e = c; e < end; ++e) to[e] = from_f32<T>(float(from[e]) * s);
@@ -531,7 +546,8 @@ extern "C" int spkv2_cuda_dequantize_rows_i8(const Spkv2DequantizeRowsI8 *a, voi
       const unsigned grid = unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64));
       return cuda_status(launch_kernel(row_values_shifted_kernel<T>, grid, 256u, 0, s, 1, a->codes, a->scale,
                                        static_cast<T *>(a->y), int(a->width), uint32_t(chunks), FastDiv(uint32_t(per_row)),
-                                       a->codes_stride, a->y_stride));
+                                       a->codes_stride, a->y_stride,
+                                       reinterpret_cast<uintptr_t>(a->codes) % 4 == 0 && (!many || a->codes_stride % 4 == 0)));
     }
     if (vw == 16) return launch_values<T, 16>(a, s);
     if (size == 2 || vw == 8) return launch_values<T, 8>(a, s);
