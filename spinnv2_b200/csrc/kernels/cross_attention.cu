@@ -23,7 +23,8 @@ using namespace xf;
 using namespace tc;
 
 // ------------------------------------------------------------ CUDA cores
-// Any type, width and alignment, exact fp32 products.  16 R rows x 64 keys a
+// What the tensor-core kernels do not take: widths over 128, and 16-bit types of odd
+// width or alignment or with a scale that is not positive.  Exact fp32 products.  16 R rows x 64 keys a
 // step, 256 threads; a thread holds scores for R rows x 4 keys and sums for R
 // rows x D / 16 columns.  The 16 threads of a row group are half a warp.  Bound
 // by the FMA pipe with four rows a thread (their operands take 12 of 16
@@ -333,11 +334,14 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   a.scale_log2 = x->scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (cross_tc_serves(a, x->dtype)) return a.rows <= 32 ? cross_step(a, x->dtype, s) : cross_tc(a, x->dtype, s);
+  if (x->dtype == SPKV2_DTYPE_FP32 && a.width <= 128) return cross_f32(a, s);
   return by_type(x->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.width <= 32) return launch_rows<T, 32>(a, s);
-    if (a.width <= 64) return launch_rows<T, 64>(a, s);
-    if (a.width <= 128) return launch_rows<T, 128>(a, s);
+    if constexpr (sizeof(T) == 2) {
+      if (a.width <= 32) return launch_rows<T, 32>(a, s);
+      if (a.width <= 64) return launch_rows<T, 64>(a, s);
+      if (a.width <= 128) return launch_rows<T, 128>(a, s);
+    }
     return launch_rows<T, 256>(a, s);
   });
 }

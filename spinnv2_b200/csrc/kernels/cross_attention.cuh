@@ -1,7 +1,8 @@
 // Arguments shared by the cross attention kernels: cross_attention.cu (CUDA
 // cores, any type and alignment, and the choice between the kernels),
-// cross_attention_tc.cu (tcgen05, 16-bit types, many rows) and
-// cross_attention_step.cu (mma.sync, 16-bit types, few rows).
+// cross_attention_tc.cu (tcgen05, 16-bit types, many rows),
+// cross_attention_step.cu (mma.sync, 16-bit types, few rows) and
+// cross_attention_f32.cu (mma.sync, fp32 by three TF32 passes).
 #pragma once
 
 #include "tcgen05.cuh"
@@ -61,5 +62,6 @@ inline bool encode_kv(KvMap *m, const AttnArgs &a, const void *base, const int64
 bool cross_tc_serves(const AttnArgs &a, int32_t dtype);
 int cross_tc(const AttnArgs &a, int32_t dtype, cudaStream_t s);
 int cross_step(const AttnArgs &a, int32_t dtype, cudaStream_t s);  // a.rows <= 32
+int cross_f32(const AttnArgs &a, cudaStream_t s);  // fp32, a.width <= 128
 
 }  // namespace spkv2

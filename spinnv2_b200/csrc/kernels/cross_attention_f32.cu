@@ -1,0 +1,367 @@
+// Cross attention in fp32 on the tensor cores (mma.sync, TF32 in three passes).
+//
+// An fp32 value x is split into hi = x rounded to TF32 and lo = x - hi, which is
+// exact and fits TF32 up to 2^-22 of x, and a product into hi hi + hi lo + lo hi;
+// what is left out is 2^-22 of it, less than fp32 sums of the same length round
+// off (850 keys of width 32: 2.0e-7 of the answer, fp32 products 4.8e-7).
+//
+// A CTA of four warps passes over the keys in tiles of 64.  W warps (1, 2 or 4)
+// share 16 of the CTA's 64 / W rows and take 64 / W of a tile's keys each, with
+// their own m, l and O, joined at the end: more where 64 rows a CTA would leave SMs
+// idle or most of the rows empty.
+// Keys and values have one buffer each: the next tile's keys load while this
+// tile's probabilities and values are multiplied, and its values during the next
+// scores.  The scores' accumulators are the next product's A operand: its columns
+// t and t + 4 stand for keys 2 t and 2 t + 1 of eight, in both operands.
+//
+// With too few row tiles for the SMs the CTAs of a cluster divide the keys, as in
+// the other kernels.  Bound by the MMAs: 45 TFLOP/s of answers (4 x 1024 x 16 heads,
+// 1024 keys, width 128: 766 us; on CUDA cores 1339 us), three TF32 MMAs each.
+#include "cross_attention.cuh"
+
+namespace spkv2 {
+
+namespace {
+
+using namespace xf;
+using namespace tc;
+
+constexpr int kKeys = 64, kThreads = 128, kMaxCluster = 8;
+
+template <int D, int W>
+struct F32Smem {
+  static constexpr int rows = 64 / W;
+  float k[kKeys][D + 4];  // at the end, with v: O, [64][D]
+  float v[kKeys][D + 4];
+  float q[rows][D + 4];
+  float m[64], l[64];  // of the warps' 16 rows
+  float cm[64], cl[64];  // of the CTA's rows, joined
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// x = hi + lo, both as TF32 operands (the low bits of lo are dropped by the MMA).
+__device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
+  const float h = tf32_rna(x);
+  hi = __float_as_uint(h);
+  lo = __float_as_uint(x - h);
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// G accumulators by one A operand and G B operands, three passes.
+template <int G>
+__device__ __forceinline__ void mma3(float (*c)[4], const float (&a)[4], const float (&b)[G][2]) {
+  uint32_t ah[4], al[4], bh[G][2], bl[G][2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split(a[e], ah[e], al[e]);
+#pragma unroll
+  for (int n = 0; n < G; ++n) {
+    split(b[n][0], bh[n][0], bl[n][0]);
+    split(b[n][1], bh[n][1], bl[n][1]);
+  }
+#pragma unroll
+  for (int n = 0; n < G; ++n) mma(c[n], al, bh[n]);
+#pragma unroll
+  for (int n = 0; n < G; ++n) mma(c[n], ah, bl[n]);
+#pragma unroll
+  for (int n = 0; n < G; ++n) mma(c[n], ah, bh[n]);
+}
+
+// 4-byte async copy global -> shared; bytes = 0 writes zeros.
+__device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int D, int W>
+__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  using S = F32Smem<D, W>;
+  S &sm = *reinterpret_cast<S *>(smem_raw);
+  constexpr int KW = 64 / W, NT = KW / 8;  // keys of a warp in a tile, in eights
+  constexpr int G = NT < 4 ? NT : 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int rank = csize > 1 ? int(cluster_rank()) : 0;
+  int item = int(blockIdx.x) / csize;
+  const int r0 = item % a.row_tiles * S::rows;
+  item /= a.row_tiles;
+  const int hk = item % a.kv_heads, b = item / a.kv_heads;
+  const float *q = static_cast<const float *>(a.q) + b * a.qs[0];
+  const float *k = static_cast<const float *>(a.k) + b * a.ks[0] + hk * a.ks[2];
+  const float *v = static_cast<const float *>(a.v) + b * a.vs[0] + hk * a.vs[2];
+  const int keys = entry_keys(a, b), tiles = (keys + kKeys - 1) / kKeys;
+  const int tile0 = int(int64_t(tiles) * rank / csize), tile1 = int(int64_t(tiles) * (rank + 1) / csize);
+
+  // A tile's keys or values; zeros for keys that do not count and beyond the width.
+  auto load = [&](float (*to)[D + 4], const float *from, int64_t stride, int tile) {
+    if (vec) {
+#pragma unroll 4
+      for (int e = tid * 4; e < kKeys * D; e += kThreads * 4) {
+        const int r = e / D, c = e % D, j = tile * kKeys + r;
+        const bool in = j < keys && c < a.width && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
+        cp_async16(&to[r][c], in ? from + j * stride + c : from, in ? 16u : 0u);
+      }
+    } else {
+#pragma unroll 4
+      for (int e = tid; e < kKeys * D; e += kThreads) {
+        const int r = e / D, c = e % D, j = tile * kKeys + r;
+        const bool in = j < keys && c < a.width && (!a.key_mask || a.key_mask[b * a.mask_stride + j] != 0);
+        cp_async4(&to[r][c], in ? from + j * stride + c : from, in ? 4u : 0u);
+      }
+    }
+  };
+  if (tile0 < tile1) load(sm.k, k, a.ks[1], tile0);
+  cp_async_commit();
+  if (tile0 < tile1) load(sm.v, v, a.vs[1], tile0);
+  cp_async_commit();
+#pragma unroll 4
+  for (int e = tid; e < S::rows * D; e += kThreads) {
+    const int r = e / D, c = e % D, row = r0 + r;
+    sm.q[r][c] = row < a.rows && c < a.width ? q[row_offset(a, a.qs, hk, row) + c] : 0.0f;
+  }
+
+  const int qr = warp / W * 16, key0 = warp % W * KW;  // this warp's rows and keys of a tile
+  float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+  for (int tile = tile0; tile < tile1; ++tile) {
+    uint64_t bits = ~uint64_t(0);  // which of the tile's keys count
+    const int j0 = tile * kKeys;
+    if (a.key_mask || j0 + kKeys > keys) {
+      bits = 0;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int j = j0 + w * 32 + lane;
+        bool in = j < keys;
+        if (in && a.key_mask) in = a.key_mask[b * a.mask_stride + j] != 0;
+        bits |= uint64_t(__ballot_sync(0xffffffffu, in)) << (32 * w);
+      }
+    }
+    cp_async_wait<1>();  // the keys; the values may still be on their way
+    __syncthreads();
+    float s[NT][4] = {};
+#pragma unroll 2
+    for (int c = 0; c < D; c += 8) {
+      const float av[4] = {sm.q[qr + g][c + t], sm.q[qr + g + 8][c + t], sm.q[qr + g][c + t + 4], sm.q[qr + g + 8][c + t + 4]};
+#pragma unroll
+      for (int n = 0; n < NT; n += G) {
+        float bv[G][2];
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          bv[i][0] = sm.k[key0 + (n + i) * 8 + g][c + t];
+          bv[i][1] = sm.k[key0 + (n + i) * 8 + g][c + t + 4];
+        }
+        mma3<G>(&s[n], av, bv);
+      }
+    }
+    __syncthreads();  // everybody has read the keys
+    if (tile + 1 < tile1) load(sm.k, k, a.ks[1], tile + 1);
+    cp_async_commit();
+
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = (bits >> (key0 + n * 8 + 2 * t + (e & 1))) & 1;
+        s[n][e] = in ? s[n][e] * a.scale_log2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      }
+    bool rise[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      rise[h] = top[h] > m[h] + 8.0f;  // from m = -inf: any score
+    }
+    if (__any_sync(0xffffffffu, rise[0] || rise[1])) {
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f[h] = rise[h] ? ex2(m[h] - top[h]) : 1.0f;
+        if (rise[h]) m[h] = top[h];
+        l[h] *= f[h];
+      }
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] *= f[e >> 1];
+    }
+    const float use[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = ex2(s[n][e] - use[e >> 1]);
+        l[e >> 1] += s[n][e];
+      }
+    cp_async_wait<1>();  // the values; the next keys may still be on their way
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float pv[4] = {s[n][0], s[n][2], s[n][1], s[n][3]};  // columns t and t + 4: keys 2 t and 2 t + 1
+      const int j = key0 + n * 8 + 2 * t;
+#pragma unroll
+      for (int d = 0; d < D / 8; d += 4) {
+        float bv[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bv[i][0] = sm.v[j][(d + i) * 8 + g];
+          bv[i][1] = sm.v[j + 1][(d + i) * 8 + g];
+        }
+        mma3<4>(&o[d], pv, bv);
+      }
+    }
+    __syncthreads();  // everybody has read the values
+    if (tile + 1 < tile1) load(sm.v, v, a.vs[1], tile + 1);
+    cp_async_commit();
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+  }
+  auto out_row = [&](int row) { return static_cast<float *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row); };
+  if (W == 1 && csize == 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + qr + h * 8 + g;
+      if (row >= a.rows) continue;
+      const float inv = l[h] != 0.0f ? 1.0f / l[h] : 0.0f;
+      float *out = out_row(row);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (n * 8 + 2 * t + e < a.width) out[n * 8 + 2 * t + e] = o[n][2 * h + e] * inv;
+    }
+    return;
+  }
+  __syncthreads();  // the last values have been read: O goes over keys and values
+  float *part = &sm.k[0][0];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = warp * 16 + h * 8 + g;
+    if (t == 0) {
+      sm.m[r] = m[h];
+      sm.l[r] = l[h];
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+      *reinterpret_cast<float2 *>(part + r * D + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+  }
+  __syncthreads();
+  auto weight = [](float mw, float top) { return mw == -INFINITY ? 0.0f : ex2(mw - top); };
+  const int used = min(S::rows, a.rows - r0) * D;
+  // Row r is rows r % 16 of the W warps from r / 16 * W on; joined in warp order into
+  // the first one's place.
+  auto place = [](int r) { return r / 16 * W * 16 + r % 16; };
+  if (W > 1) {
+    for (int e = tid; e < used; e += kThreads) {
+      const int r = e / D, c = e % D, at = place(r);
+      float top = sm.m[at], acc = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[at + w * 16]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = weight(sm.m[at + w * 16], top);
+        acc = fmaf(part[(at + w * 16) * D + c], f, acc);
+        sum = fmaf(sm.l[at + w * 16], f, sum);
+      }
+      if (csize == 1) {
+        if (c < a.width) out_row(r0 + r)[c] = sum != 0.0f ? acc / sum : 0.0f;
+      } else {
+        part[at * D + c] = acc;
+        if (c == 0) {
+          sm.cm[r] = top;
+          sm.cl[r] = sum;
+        }
+      }
+    }
+  }
+  if (csize > 1) {
+    const float *cm = W > 1 ? sm.cm : sm.m, *cl = W > 1 ? sm.cl : sm.l;
+    __syncwarp();
+    cluster_sync();
+    for (int e = rank * kThreads + tid; e < used; e += csize * kThreads) {
+      const int r = e / D, c = e % D;
+      float mk[kMaxCluster], lk[kMaxCluster], ok[kMaxCluster], top = -INFINITY, acc = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kMaxCluster; ++n) {
+        if (n >= csize) break;
+        mk[n] = __uint_as_float(ld_cluster(map_rank(&cm[r], n)));
+        lk[n] = __uint_as_float(ld_cluster(map_rank(&cl[r], n)));
+        ok[n] = __uint_as_float(ld_cluster(map_rank(&part[place(r) * D + c], n)));
+        top = fmaxf(top, mk[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < kMaxCluster; ++n) {
+        if (n >= csize) break;
+        const float f = weight(mk[n], top);
+        acc = fmaf(ok[n], f, acc);
+        sum = fmaf(lk[n], f, sum);
+      }
+      if (c < a.width) out_row(r0 + r)[c] = sum != 0.0f ? acc / sum : 0.0f;
+    }
+    __syncwarp();
+    cluster_sync();  // the peers have read this CTA's sums
+  }
+}
+
+template <int D, int W>
+int launch(AttnArgs a, int csize, cudaStream_t s) {
+  using S = F32Smem<D, W>;
+  static_assert(sizeof(S::k) + sizeof(S::v) >= 64 * D * 4, "O takes the place of keys and values");
+  a.row_tiles = int(ceil_div(a.rows, S::rows));
+  const int64_t blocks = int64_t(a.row_tiles) * a.kv_heads * a.batch;
+  if (blocks * csize > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
+  if (const int rc = allow_smem<cross_f32_kernel<D, W>>(sizeof(S))) return rc;
+  auto rows16 = [](const void *base, const int64_t (&st)[3]) {
+    return aligned16(base) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+  };
+  const bool vec = a.width % 4 == 0 && rows16(a.k, a.ks) && rows16(a.v, a.vs);
+  return cuda_status(launch_kernel(cross_f32_kernel<D, W>, unsigned(blocks * csize), unsigned(kThreads), sizeof(S), s, csize, a,
+                                   csize, vec));
+}
+
+// Warps a row and CTAs a cluster by an estimate of the time in microseconds, fitted
+// to sweeps of both over ten sizes (the choice took at most 25 % longer than the
+// best): a tile takes its warps `wait` + `work` / W one after another, and an SM
+// `share` + `full` / W of its throughput; a cluster of eight is slow to start where
+// there are more CTAs than SMs.
+template <int D>
+int launch_rows(const AttnArgs &a, cudaStream_t s) {
+  constexpr double wait = D == 32 ? 1.5 : D == 64 ? 3.1 : 3.6, work = D == 32 ? 0.7 : D == 64 ? 1.6 : 5.2;
+  constexpr double share = D == 32 ? 0.3 : D == 64 ? 0.7 : 1.4, full = D == 32 ? 2.2 : D == 64 ? 2.6 : 5.5;
+  const double sms = sm_count();
+  const int64_t tiles = ceil_div(a.keys, kKeys);
+  int best_w = 1, best_c = 1;
+  double best = 1e30;
+  for (int w = 1; w <= 4; w *= 2)
+    for (int c = 1; c <= kMaxCluster && (c == 1 || tiles >= c); c *= 2) {
+      const double ctas = double(ceil_div(a.rows, 64 / w)) * a.kv_heads * a.batch * c, each = double(ceil_div(tiles, c));
+      const double start = c == 1 ? 0.0 : c == 2 ? 1.0 : c == 4 ? 2.0 : 3.0 + 3.0 * std::max(0.0, ctas / sms - 1.0);
+      const double time = start + std::max(3.0 + each * (wait + work / w), ctas * each * (share + full / w) / sms);
+      if (time < best) best = time, best_w = w, best_c = c;
+    }
+  if (best_w == 4) return launch<D, 4>(a, best_c, s);
+  return best_w == 2 ? launch<D, 2>(a, best_c, s) : launch<D, 1>(a, best_c, s);
+}
+
+}  // namespace
+
+int cross_f32(const AttnArgs &a, cudaStream_t s) {
+  if (a.width <= 32) return launch_rows<32>(a, s);
+  return a.width <= 64 ? launch_rows<64>(a, s) : launch_rows<128>(a, s);
+}
+
+}  // namespace spkv2
