@@ -24,14 +24,13 @@ using namespace tc;
 
 // ------------------------------------------------------------ CUDA cores
 // What the tensor-core kernels do not take: widths over 128, and 16-bit types of odd
-// width or alignment or with a scale that is not positive.  Exact fp32 products.  16 R rows x 64 keys a
-// step, 256 threads; a thread holds scores for R rows x 4 keys and sums for R
-// rows x D / 16 columns.  The 16 threads of a row group are half a warp.  Bound
-// by the FMA pipe with four rows a thread (their operands take 12 of 16
-// shared-memory cycles); with few rows by shared memory, which every warp reads
-// whole for its two rows.  With too few row tiles for the SMs the CTAs of a
-// cluster divide the keys and join their m, l and O through distributed shared
-// memory, in CTA order.
+// width or alignment or with a scale that is not positive.  Exact fp32 products.
+// 16 R rows x 64 keys a step, 256 threads; a thread holds scores for R rows x 4 keys
+// and sums for R rows x D / 16 columns.  The 16 threads of a row group are half a
+// warp.  Bound by issue and the FMA pipe with four rows a thread (25 TFLOP/s at width
+// 128); with few rows by shared memory, which every warp reads whole for its two
+// rows.  With too few row tiles for the SMs the CTAs of a cluster divide the keys and
+// join their m, l and O through distributed shared memory, in CTA order.
 constexpr int kKeys = 64, kMaxCluster = 8;
 
 template <int D, int R>

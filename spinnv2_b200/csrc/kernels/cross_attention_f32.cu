@@ -2,8 +2,10 @@
 //
 // An fp32 value x is split into hi = x rounded to TF32 and lo = x - hi, which is
 // exact and fits TF32 up to 2^-22 of x, and a product into hi hi + hi lo + lo hi;
-// what is left out is 2^-22 of it, less than fp32 sums of the same length round
-// off (850 keys of width 32: 2.0e-7 of the answer, fp32 products 4.8e-7).
+// what is left out is 2^-22 of it.  The MMA cuts its sums off where fp32 would round
+// them, which adds up over long chains (2e-6 of the answer); so a sum takes four
+// (scores) or eight (answers) MMAs from zero and is then added up in fp32 registers,
+// and the small cross products have sums of their own.
 //
 // A CTA of four warps passes over the keys in tiles of 64.  W warps (1, 2 or 4)
 // share 16 of the CTA's 64 / W rows and take 64 / W of a tile's keys each, with
@@ -15,8 +17,9 @@
 // t and t + 4 stand for keys 2 t and 2 t + 1 of eight, in both operands.
 //
 // With too few row tiles for the SMs the CTAs of a cluster divide the keys, as in
-// the other kernels.  Bound by the MMAs: 45 TFLOP/s of answers (4 x 1024 x 16 heads,
-// 1024 keys, width 128: 766 us; on CUDA cores 1339 us), three TF32 MMAs each.
+// the other kernels.  Bound by the MMAs and what splits their operands: 40 TFLOP/s of
+// answers (4 x 1024 x 16 heads, 1024 keys, width 128: 862 us; on CUDA cores 1339 us),
+// three TF32 MMAs each.
 #include "cross_attention.cuh"
 
 namespace spkv2 {
@@ -57,9 +60,10 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// G accumulators by one A operand and G B operands, three passes.
+// G accumulators by one A operand and G B operands: the large products into c, the
+// cross products, 2^-11 of them, into their own sums.
 template <int G>
-__device__ __forceinline__ void mma3(float (*c)[4], const float (&a)[4], const float (&b)[G][2]) {
+__device__ __forceinline__ void mma3(float (&c)[G][4], float (&cross)[G][4], const float (&a)[4], const float (&b)[G][2]) {
   uint32_t ah[4], al[4], bh[G][2], bl[G][2];
 #pragma unroll
   for (int e = 0; e < 4; ++e) split(a[e], ah[e], al[e]);
@@ -69,11 +73,11 @@ __device__ __forceinline__ void mma3(float (*c)[4], const float (&a)[4], const f
     split(b[n][1], bh[n][1], bl[n][1]);
   }
 #pragma unroll
-  for (int n = 0; n < G; ++n) mma(c[n], al, bh[n]);
-#pragma unroll
-  for (int n = 0; n < G; ++n) mma(c[n], ah, bl[n]);
-#pragma unroll
   for (int n = 0; n < G; ++n) mma(c[n], ah, bh[n]);
+#pragma unroll
+  for (int n = 0; n < G; ++n) mma(cross[n], al, bh[n]);
+#pragma unroll
+  for (int n = 0; n < G; ++n) mma(cross[n], ah, bl[n]);
 }
 
 // 4-byte async copy global -> shared; bytes = 0 writes zeros.
@@ -82,7 +86,7 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t b
 }
 
 template <int D, int W>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec) {
+__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using S = F32Smem<D, W>;
   S &sm = *reinterpret_cast<S *>(smem_raw);
@@ -148,18 +152,26 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) cross_f32_kernel(A
     cp_async_wait<1>();  // the keys; the values may still be on their way
     __syncthreads();
     float s[NT][4] = {};
-#pragma unroll 2
-    for (int c = 0; c < D; c += 8) {
-      const float av[4] = {sm.q[qr + g][c + t], sm.q[qr + g + 8][c + t], sm.q[qr + g][c + t + 4], sm.q[qr + g + 8][c + t + 4]};
 #pragma unroll
-      for (int n = 0; n < NT; n += G) {
-        float bv[G][2];
+    for (int n = 0; n < NT; n += G) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        float sum[G][4] = {}, cross[G][4] = {};
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-          bv[i][0] = sm.k[key0 + (n + i) * 8 + g][c + t];
-          bv[i][1] = sm.k[key0 + (n + i) * 8 + g][c + t + 4];
+        for (int c = c0; c < c0 + 32; c += 8) {
+          const float av[4] = {sm.q[qr + g][c + t], sm.q[qr + g + 8][c + t], sm.q[qr + g][c + t + 4], sm.q[qr + g + 8][c + t + 4]};
+          float bv[G][2];
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            bv[i][0] = sm.k[key0 + (n + i) * 8 + g][c + t];
+            bv[i][1] = sm.k[key0 + (n + i) * 8 + g][c + t + 4];
+          }
+          mma3<G>(sum, cross, av, bv);
         }
-        mma3<G>(&s[n], av, bv);
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n + i][e] += sum[i][e] + cross[i][e];
       }
     }
     __syncthreads();  // everybody has read the keys
@@ -206,19 +218,24 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) cross_f32_kernel(A
     cp_async_wait<1>();  // the values; the next keys may still be on their way
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float pv[4] = {s[n][0], s[n][2], s[n][1], s[n][3]};  // columns t and t + 4: keys 2 t and 2 t + 1
-      const int j = key0 + n * 8 + 2 * t;
+    for (int d = 0; d < D / 8; d += 4) {
+      float sum[4][4] = {}, cross[4][4] = {};
 #pragma unroll
-      for (int d = 0; d < D / 8; d += 4) {
+      for (int n = 0; n < NT; ++n) {
+        const float pv[4] = {s[n][0], s[n][2], s[n][1], s[n][3]};  // columns t and t + 4: keys 2 t and 2 t + 1
+        const int j = key0 + n * 8 + 2 * t;
         float bv[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           bv[i][0] = sm.v[j][(d + i) * 8 + g];
           bv[i][1] = sm.v[j + 1][(d + i) * 8 + g];
         }
-        mma3<4>(&o[d], pv, bv);
+        mma3<4>(sum, cross, pv, bv);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d + i][e] += sum[i][e] + cross[i][e];
     }
     __syncthreads();  // everybody has read the values
     if (tile + 1 < tile1) load(sm.v, v, a.vs[1], tile + 1);
