@@ -30,8 +30,7 @@ using namespace tc;
 constexpr int kTile = 128;  // rows of a tile, keys of a step
 constexpr int kHalf = kTile * 128;  // bytes of 64 columns of a tile
 
-// TILES: row tiles of a CTA.  Two for many rows (one CTA per SM); one, with two
-// CTAs per SM, where there are fewer CTAs of two tiles than SMs.
+// TILES: row tiles of a CTA: two, with one CTA per SM, or one with two CTAs.
 template <int D, int TILES>
 struct Shape {
   static constexpr int halves = D / 64;
@@ -114,7 +113,8 @@ __device__ __forceinline__ void key_bits(const AttnArgs &a, int b, int keys, int
 
 template <class T, int D, int TILES>
 __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
-    cross_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a,
+    cross_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, AttnArgs a, bool q_tma,
                     int k_heads_step, int k_batch_step, int v_heads_step, int v_batch_step, int csize) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    mbar_init(&q_bar, SOFT);
+    mbar_init(&q_bar, q_tma ? 1 : SOFT);
     mbar_init(&done_bar, 1);
     for (int i = 0; i < TILES; ++i) {
       mbar_init(&s_bar[i], 1);
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::soft_regs));
     const int i = warp >> 2, quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    {  // this warp's 32 rows of Q, swizzled for the MMA; 16-byte chunks
+    if (!q_tma) {  // this warp's 32 rows of Q, swizzled for the MMA; 16-byte chunks
       const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
       constexpr int CH = D / 8, RPI = 32 / CH;  // chunks of a row, rows of an iteration
       const int c = lane % CH;
@@ -316,6 +316,12 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
     // ---------------------------------------------------------- K and V tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::other_regs));
     if (warp == SOFT && elect_one()) {
+      if (q_tma) {
+        mbar_arrive_expect_tx(&q_bar, uint32_t(tiles * S::tile_bytes));
+        for (int i = 0; i < tiles; ++i)
+          for (int h = 0; h < S::halves; ++h)
+            tma_load_4d(smem + i * S::tile_bytes + h * kHalf, &qmap, h * 64, hk * a.group, (r0 + i * kTile) / a.group, b, &q_bar);
+      }
       int it = 0;
       bool ok = true;
       for (int j = 0; j < steps && ok; ++j) {
@@ -330,6 +336,11 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
         }
       }
       // What was issued has landed before shared memory goes away.
+      if (q_tma) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&q_bar, 0) && clock64() - t0 < kWaitCycles) {
+        }
+      }
       for (int k = it > S::slots ? it - S::slots : 0; k < it; ++k) {
         const long long t0 = clock64();
         while (!mbar_try_wait(&full_bar[k % S::slots], (k / S::slots) & 1) && clock64() - t0 < kWaitCycles) {
@@ -469,6 +480,25 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
   }
 }
 
+// Q as {width, head, token, entry}: where the heads of a group divide the 128 rows
+// of a tile, the tile is a box of group heads x 128 / group tokens, in the order of
+// the rows.
+bool encode_q(CUtensorMap *map, const AttnArgs &a) {
+  const int64_t heads = int64_t(a.kv_heads) * a.group, most = int64_t(1) << 38;
+  if (kTile % a.group != 0) return false;
+  if ((heads > 1 && a.qs[2] <= 0) || (a.queries > 1 && a.qs[1] <= 0) || (a.batch > 1 && a.qs[0] <= 0)) return false;
+  if (a.qs[0] >= most || a.qs[1] >= most || a.qs[2] >= most) return false;
+  const cuuint64_t any = (cuuint64_t(a.width) * 2 + 15) / 16 * 16;
+  const cuuint64_t dims[4] = {cuuint64_t(a.width), cuuint64_t(heads), cuuint64_t(a.queries), cuuint64_t(a.batch)};
+  const cuuint64_t strides[3] = {heads > 1 ? cuuint64_t(a.qs[2]) * 2 : any, a.queries > 1 ? cuuint64_t(a.qs[1]) * 2 : any,
+                                 a.batch > 1 ? cuuint64_t(a.qs[0]) * 2 : any};
+  const cuuint32_t box[4] = {64, cuuint32_t(a.group), cuuint32_t(kTile / a.group), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(a.q), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class T, int D, int TILES>
 int launch(AttnArgs a, cudaStream_t s) {
   using S = Shape<D, TILES>;
@@ -478,19 +508,25 @@ int launch(AttnArgs a, cudaStream_t s) {
   if (const int rc = allow_smem<cross_tc_kernel<T, D, TILES>>(S::smem)) return rc;
   KvMap k, v;
   if (!encode_kv(&k, a, a.k, a.ks, kTile) || !encode_kv(&v, a, a.v, a.vs, kTile)) return SPKV2_ERR_CUDA;
+  CUtensorMap qmap = {};
+  const bool q_tma = encode_q(&qmap, a);
   // Too few tiles for the SMs: divide the keys, down to two steps a CTA.
   int csize = 1;
   if (TILES == 1)
     while (csize < kMaxCluster && blocks * csize * 2 <= 2 * sm_count() && ceil_div(a.keys, kTile) >= 4 * csize) csize *= 2;
   if (blocks * csize > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  return cuda_status(launch_kernel(cross_tc_kernel<T, D, TILES>, unsigned(blocks * csize), S::threads, S::smem, s, csize, k.map,
-                                   v.map, a, k.heads_step, k.batch_step, v.heads_step, v.batch_step, csize));
+  return cuda_status(launch_kernel(cross_tc_kernel<T, D, TILES>, unsigned(blocks * csize), S::threads, S::smem, s, csize, qmap,
+                                   k.map, v.map, a, q_tma, k.heads_step, k.batch_step, v.heads_step, v.batch_step, csize));
 }
 
 template <class T, int D>
 int launch_tiles(const AttnArgs &a, cudaStream_t s) {
+  // Two tiles for long passes over the keys that fill the SMs; else two CTAs an SM,
+  // so that one works while the other starts or ends (width 128, 16 x 16 heads x
+  // 1024 rows: 4096 keys 455 us against 492, 1024 keys 177 us against 167, 256 keys
+  // 98 against 82).
   const int64_t blocks = ceil_div(a.rows, 2 * kTile) * a.kv_heads * a.batch;
-  return a.rows > kTile && blocks >= sm_count() ? launch<T, D, 2>(a, s) : launch<T, D, 1>(a, s);
+  return a.rows > kTile && blocks >= sm_count() && a.keys >= 2048 ? launch<T, D, 2>(a, s) : launch<T, D, 1>(a, s);
 }
 
 bool rows_aligned(const void *base, const int64_t (&st)[3]) {

@@ -307,7 +307,8 @@ SHAPES = [  # batch, queries, keys, heads, kv_heads, width
     (1, 2, 300, 64, 2, 32), (2, 64, 128, 3, 3, 64), (1, 65, 257, 4, 4, 128), (1, 100, 850, 8, 8, 32), (2, 77, 196, 12, 12, 64),
     (1, 128, 1, 2, 2, 64), (1, 129, 384, 2, 1, 128), (2, 300, 200, 4, 2, 64), (1, 257, 1025, 8, 2, 128), (1, 31, 33, 5, 5, 7),
     (1, 40, 70, 2, 2, 130), (2, 1, 90, 4, 2, 256), (1, 33, 129, 2, 1, 200), (1, 600, 513, 3, 3, 96), (1, 1, 20000, 2, 2, 64),
-    (70, 1, 3, 2, 1, 16), (1, 130, 129, 2, 2, 8), (3, 5, 0, 2, 2, 64)]
+    (70, 1, 3, 2, 1, 16), (1, 130, 129, 2, 2, 8), (3, 5, 0, 2, 2, 64),
+    (20, 400, 300, 4, 4, 128), (10, 130, 129, 32, 8, 96), (40, 450, 64, 2, 2, 128), (19, 513, 640, 4, 4, 104)]
 
 
 @gpu_test
