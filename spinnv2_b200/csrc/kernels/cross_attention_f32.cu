@@ -86,7 +86,7 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t b
 }
 
 template <int D, int W>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec) {
+__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec, bool vec_q, bool vec_out) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using S = F32Smem<D, W>;
   S &sm = *reinterpret_cast<S *>(smem_raw);
@@ -124,15 +124,25 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
       }
     }
   };
+  if (vec_q) {
+#pragma unroll 4
+    for (int e = tid * 4; e < S::rows * D; e += kThreads * 4) {
+      const int r = e / D, c = e % D, row = r0 + r;
+      const bool in = row < a.rows && c < a.width;
+      cp_async16(&sm.q[r][c], in ? q + row_offset(a, a.qs, hk, row) + c : q, in ? 16u : 0u);
+    }
+  } else {
+#pragma unroll 4
+    for (int e = tid; e < S::rows * D; e += kThreads) {
+      const int r = e / D, c = e % D, row = r0 + r;
+      const bool in = row < a.rows && c < a.width;
+      cp_async4(&sm.q[r][c], in ? q + row_offset(a, a.qs, hk, row) + c : q, in ? 4u : 0u);
+    }
+  }
   if (tile0 < tile1) load(sm.k, k, a.ks[1], tile0);
   cp_async_commit();
   if (tile0 < tile1) load(sm.v, v, a.vs[1], tile0);
   cp_async_commit();
-#pragma unroll 4
-  for (int e = tid; e < S::rows * D; e += kThreads) {
-    const int r = e / D, c = e % D, row = r0 + r;
-    sm.q[r][c] = row < a.rows && c < a.width ? q[row_offset(a, a.qs, hk, row) + c] : 0.0f;
-  }
 
   const int qr = warp / W * 16, key0 = warp % W * KW;  // this warp's rows and keys of a tile
   float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
@@ -149,11 +159,13 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
         bits |= uint64_t(__ballot_sync(0xffffffffu, in)) << (32 * w);
       }
     }
+    const int live = keys - j0 - key0;  // this warp's keys of the tile end here: eights beyond are skipped
     cp_async_wait<1>();  // the keys; the values may still be on their way
     __syncthreads();
     float s[NT][4] = {};
 #pragma unroll
     for (int n = 0; n < NT; n += G) {
+      if (n * 8 >= live) break;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
         float sum[G][4] = {}, cross[G][4] = {};
@@ -222,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
       float sum[4][4] = {}, cross[4][4] = {};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (n * 8 >= live) break;
         const float pv[4] = {s[n][0], s[n][2], s[n][1], s[n][3]};  // columns t and t + 4: keys 2 t and 2 t + 1
         const int j = key0 + n * 8 + 2 * t;
         float bv[4][2];
@@ -256,10 +269,16 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
       const float inv = l[h] != 0.0f ? 1.0f / l[h] : 0.0f;
       float *out = out_row(row);
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (n * 8 + 2 * t + e < a.width) out[n * 8 + 2 * t + e] = o[n][2 * h + e] * inv;
+      for (int n = 0; n < D / 8; ++n) {
+        const int c = n * 8 + 2 * t;
+        const float x = o[n][2 * h] * inv, y = o[n][2 * h + 1] * inv;
+        if (vec_out) {
+          if (c < a.width) *reinterpret_cast<float2 *>(out + c) = make_float2(x, y);
+        } else {
+          if (c < a.width) out[c] = x;
+          if (c + 1 < a.width) out[c + 1] = y;
+        }
+      }
     }
     return;
   }
@@ -346,8 +365,10 @@ int launch(AttnArgs a, int csize, cudaStream_t s) {
     return aligned16(base) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
   };
   const bool vec = a.width % 4 == 0 && rows16(a.k, a.ks) && rows16(a.v, a.vs);
+  const bool vec_q = a.width % 4 == 0 && rows16(a.q, a.qs);
+  const bool vec_out = a.width % 2 == 0 && on_bytes(8, a.out) && a.os[0] % 2 == 0 && a.os[1] % 2 == 0 && a.os[2] % 2 == 0;
   return cuda_status(launch_kernel(cross_f32_kernel<D, W>, unsigned(blocks * csize), unsigned(kThreads), sizeof(S), s, csize, a,
-                                   csize, vec));
+                                   csize, vec, vec_q, vec_out));
 }
 
 // Warps a row and CTAs a cluster by an estimate of the time in microseconds, fitted
