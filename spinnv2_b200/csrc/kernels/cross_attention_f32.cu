@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
   const float *q = static_cast<const float *>(a.q) + b * a.qs[0];
   const float *k = static_cast<const float *>(a.k) + b * a.ks[0] + hk * a.ks[2];
   const float *v = static_cast<const float *>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  const int keys = entry_keys(a, b), tiles = (keys + kKeys - 1) / kKeys;
+  const int keys = counted_keys<kThreads>(a, b, tid), tiles = (keys + kKeys - 1) / kKeys;
   const int tile0 = int(int64_t(tiles) * rank / csize), tile1 = int(int64_t(tiles) * (rank + 1) / csize);
 
   // A tile's keys or values; zeros for keys that do not count and beyond the width.

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? (D == 64 ? 4 : 3) : 2)
   pdl_launch_dependents();
   pdl_wait();
 
-  const int keys = entry_keys(a, b);
+  const int keys = counted_keys<kThreads>(a, b, tid);
   const int chunks = (keys + kChunk - 1) / kChunk;
   const int first = int(int64_t(chunks) * rank / csize) + warp;
   const int last = int(int64_t(chunks) * (rank + 1) / csize);  // this warp's chunks: first, first + 4, .. below last

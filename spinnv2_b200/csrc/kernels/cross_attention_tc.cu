@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
   pdl_launch_dependents();
   pdl_wait();
 
-  const int keys = entry_keys(a, b);
+  const int keys = counted_keys<S::threads>(a, b, tid);
   const int all_steps = (keys + kTile - 1) / kTile;  // divided among the CTAs of the cluster
   const int step0 = int(int64_t(all_steps) * rank / csize), steps = int(int64_t(all_steps) * (rank + 1) / csize) - step0;
   // TMEM columns: scores (and P) of tile i at 128 i, sums of tile i behind them.

@@ -406,6 +406,33 @@ def test_attention_scores_of_any_size(gpu, dtype, lq):
 
 
 @gpu_test
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lq", [1, 100])
+def test_attention_masks_that_end_early(gpu, lq, dtype):
+    """Masks over many keys whose last key that counts lies anywhere: the first, the last, around the steps of
+    the kernels, or nowhere; together with lengths."""
+    from spinnv2_b200 import transformer as T
+
+    ends = [0, 1, 16, 127, 128, 129, 2047, 2048, 2049, 4100, 4999, 5000]
+    q, k, v = inputs(len(ends), lq, 5000, 4, 2, 64, dtype, 11)
+    mask = torch.rand(len(ends), 5000, generator=gen(12), device="cuda") < 0.3
+    for i, end in enumerate(ends):
+        mask[i, end:] = False
+        if end:
+            mask[i, end - 1] = True
+    off = ~mask
+    k, v = k.clone(), v.clone()
+    k[off] = math.nan
+    v[off] = math.nan
+    check_attention(T.cross_attention(q, k, v, key_mask=mask), q, k, v, mask, 0.125)
+    lengths = torch.tensor([5000, 5000, 3, 5000, 100, 5000, 600, 513, 512, 511, 5000, 2500], dtype=torch.int32, device="cuda")
+    both = mask & (torch.arange(5000, device="cuda")[None, :] < lengths[:, None])
+    out = T.cross_attention(q, k, v, key_mask=mask, lengths=lengths)
+    check_attention(out, q, k, v, both, 0.125)
+    assert not out[0].any()
+
+
+@gpu_test
 @pytest.mark.parametrize("lq", [1, 40])
 def test_attention_offsets_past_32_bits(gpu, lq):
     from spinnv2_b200 import transformer as T
