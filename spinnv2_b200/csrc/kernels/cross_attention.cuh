@@ -35,19 +35,14 @@ __device__ __forceinline__ int entry_keys(const AttnArgs &p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
 }
 
-// The keys up to the last one of entry b that counts; called by all of a block's
-// threads.  A mask's end is searched from behind, 16 keys a thread at a time: images
-// padded to one grid end in keys that do not count (bf16, 4 x 200 rows x 16/4 heads,
-// grids within 60 x 60: 37.7 us reading every key, 19.1 so; 8 x 2 rows x 16/8 heads
-// within 43 x 87: 38.1 and 29.3).  Masks of under 512 keys are a few steps at most and
-// are not searched.
+// The end of a long mask: one past its last key that counts, searched from behind, 16
+// keys a thread at a time, by all of a block's threads.  Its own function, so that its
+// instructions lie outside the path of calls that do not search (12 heads x 77 rows
+// over 196 masked keys: 8.5 us inlined, 8.2 so).
 template <int THREADS>
-__device__ __forceinline__ int counted_keys(const AttnArgs &p, int b, int tid) {
-  const int keys = entry_keys(p, b);
-  if (!p.key_mask || keys < 512) return keys;
+__device__ __noinline__ int mask_end(const uint8_t *mask, int keys, int tid) {
   __shared__ int s_last;
   if (tid == 0) s_last = 0;
-  const uint8_t *mask = p.key_mask + b * p.mask_stride;
   constexpr int SPAN = THREADS * 16;
   int last = 0;
   for (int end = keys; end > 0; end -= SPAN) {
@@ -66,6 +61,17 @@ __device__ __forceinline__ int counted_keys(const AttnArgs &p, int b, int tid) {
   if ((tid & 31) == 0 && last) atomicMax(&s_last, last);
   __syncthreads();
   return s_last;
+}
+
+// The keys of entry b that have to be read.  Images padded to one grid end in keys that
+// do not count (bf16, 4 x 200 rows x 16/4 heads, grids within 60 x 60: 37.8 us reading
+// every key, 18.5 so; 8 x 2 rows x 16/8 heads within 43 x 87: 38.1 and 29.8).  Masks of
+// under 512 keys are a few steps at most and are not searched.
+template <int THREADS>
+__device__ __forceinline__ int counted_keys(const AttnArgs &p, int b, int tid) {
+  const int keys = entry_keys(p, b);
+  if (!p.key_mask || keys < 512) return keys;
+  return mask_end<THREADS>(p.key_mask + b * p.mask_stride, keys, tid);
 }
 
 // Tensor map of keys or values as {width, key, head, entry}, 128-byte swizzle,
