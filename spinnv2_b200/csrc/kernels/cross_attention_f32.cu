@@ -18,7 +18,7 @@
 //
 // With too few row tiles for the SMs the CTAs of a cluster divide the keys, as in
 // the other kernels.  Bound by the MMAs and what splits their operands: 40 TFLOP/s of
-// answers (4 x 1024 x 16 heads, 1024 keys, width 128: 862 us; on CUDA cores 1339 us),
+// answers (4 x 1024 x 16 heads, 1024 keys, width 128: 852 us; on CUDA cores 1339 us),
 // three TF32 MMAs each.
 #include "cross_attention.cuh"
 
