@@ -169,6 +169,8 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
   auto s_col = [&](int i) { return tmem + uint32_t(i * kTile); };
   auto o_col = [&](int i) { return tmem + uint32_t(TILES * kTile + i * D); };
 
+  // A CTA without steps loads no Q: it writes its zeros over Q's place without a wait,
+  // for peers that multiply them by 0, and what landed there later would reach them.
   float *part = reinterpret_cast<float *>(smem);  // O for the cluster's join, [tile][column][row], over Q, K and V
   auto out_row = [&](int row) {
     return static_cast<T *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row);
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::soft_regs));
     const int i = warp >> 2, quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    if (!q_tma) {  // this warp's 32 rows of Q, swizzled for the MMA; 16-byte chunks
+    if (!q_tma && steps > 0) {  // this warp's 32 rows of Q, swizzled for the MMA; 16-byte chunks
       const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
       constexpr int CH = D / 8, RPI = 32 / CH;  // chunks of a row, rows of an iteration
       const int c = lane % CH;
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
     // ---------------------------------------------------------- K and V tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::other_regs));
     if (warp == SOFT && elect_one()) {
-      if (q_tma) {
+      if (q_tma && steps > 0) {
         mbar_arrive_expect_tx(&q_bar, uint32_t(tiles * S::tile_bytes));
         for (int i = 0; i < tiles; ++i)
           for (int h = 0; h < S::halves; ++h)
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
         }
       }
       // What was issued has landed before shared memory goes away.
-      if (q_tma) {
+      if (q_tma && steps > 0) {
         const long long t0 = clock64();
         while (!mbar_try_wait(&q_bar, 0) && clock64() - t0 < kWaitCycles) {
         }
@@ -364,8 +366,8 @@ __global__ void __launch_bounds__(Shape<D, TILES>::threads, 3 - TILES)
         mma_f16(s_col(i), dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
       }
     };
-    bool ok = __all_sync(0xffffffffu, mbar_wait(&q_bar, 0, &abort_flag, status, 3));
-    if (ok && steps > 0) {
+    bool ok = steps > 0 && __all_sync(0xffffffffu, mbar_wait(&q_bar, 0, &abort_flag, status, 3));
+    if (ok) {
       ok = landed(0);
       if (ok && elect_one()) {
         tc_fence_after();
