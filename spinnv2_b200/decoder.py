@@ -81,7 +81,11 @@ def encoder_package(config: str = "resnet50", batch: int = 1) -> bytes:
 
 
 class ImageEncoder:
-    """Features of images on the device, by the graph runtime."""
+    """Features of images on the device, by the graph runtime.
+
+    The runtime writes one buffer on a stream of its own; `free` marks where torch's work on that buffer ends,
+    and each run waits for it.
+    """
 
     def __init__(self, config: str = "resnet50", batch: int = 1, *, device: int = 0) -> None:
         from .runtime import Runtime
@@ -90,12 +94,20 @@ class ImageEncoder:
         shape = self.rt.package.outputs[1].shape  # [batch, channels, height, width]
         self.features = torch.empty(tuple(shape), device=f"cuda:{device}")
         self.rt.bind_output(1, self.features.data_ptr())  # written in place, no copy
+        self.stream = torch.cuda.ExternalStream(self.rt.stream(), device=self.features.device)
+        self.free = torch.cuda.Event()
+        # Work that is queued may still use the block that the buffer lies in.
+        self.free.record(torch.cuda.current_stream(self.features.device))
 
     def __call__(self, images: np.ndarray) -> torch.Tensor:
-        """[batch, positions, channels] float32 of images [batch, 3, 224, 224]."""
+        """[batch, positions, channels] float32 of images [batch, 3, 224, 224], a tensor of its own, on
+        torch's current stream."""
         self.rt.set_input(0, images)
+        self.stream.wait_event(self.free)
         self.rt.run()  # returns when the features are written
-        return self.features.flatten(2).transpose(1, 2).contiguous()
+        answer = self.features.flatten(2).transpose(1, 2).clone(memory_format=torch.contiguous_format)
+        self.free.record(torch.cuda.current_stream(self.features.device))
+        return answer
 
     def close(self) -> None:
         self.rt.close()

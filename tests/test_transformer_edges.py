@@ -39,3 +39,41 @@ def test_query_that_is_not_finite_stays_alone(gpu, lq, hq, hk, d, dtype):
                     assert not got[lengths == 0].any()
                     got[:, at, hq - 1] = want[:, at, hq - 1]
                     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ streams
+@gpu_test
+def test_encoder_calls_behind_queued_work(gpu):
+    """An answer of the encoder holds its own images' features, also where torch's stream is still busy with
+    earlier work when the next call writes the runtime's buffer, and from one current stream to another."""
+    from conftest import seeded_input
+    from spinnv2_b200.decoder import ImageEncoder
+
+    first, second = (seeded_input((1, 3, 224, 224), seed=i) for i in (1, 2))
+    matrix = torch.randn(8192, 8192, generator=gen(1), device="cuda")
+    out = torch.empty_like(matrix)
+
+    def busy():
+        for _ in range(10):  # some 0.2 s
+            torch.mm(matrix, matrix, out=out)
+
+    busy()
+    encoder = ImageEncoder("resnet50", 1)
+    torch.cuda.synchronize()
+    want = []
+    for images in (first, second):
+        want.append(encoder(images))
+        torch.cuda.synchronize()
+    assert not torch.equal(*want)
+    busy()
+    got = [encoder(first), encoder(second)]
+    assert got[0].data_ptr() != encoder.features.data_ptr() and got[0].is_contiguous()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    busy()
+    a = encoder(first)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        b = encoder(second)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    encoder.close()
