@@ -48,7 +48,8 @@ extern "C" {
  * and bfloat16, which packages do not hold. */
 #define SPKV2_CUDA_DTYPE_BF16 16
 
-/* linear_i8's activation: the codes of the fused activations of a Conv. */
+/* linear_i8's activation: the codes of the fused activations of a Conv.  ReLU
+ * keeps a NaN. */
 #define SPKV2_CUDA_ACT_NONE 0
 #define SPKV2_CUDA_ACT_RELU 1
 #define SPKV2_CUDA_ACT_SILU 2

@@ -25,8 +25,22 @@ struct LinearArgs {
   int y_tma;  // y can be stored by TMA
 };
 
+// The activations of a Conv, but for ReLU of a NaN, which stays one here: the scale of
+// a row that was not finite has to show in what is made of it.
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+  if (act == SPKV2_CUDA_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = v[j] <= 0.0f ? 0.0f : v[j];
+  } else {
+    apply_act_n<N>(v, act);
+  }
+}
+
 __device__ __forceinline__ float linear_value(int acc, float sa, float sw, float bias, int act) {
-  return apply_act(fmaf(float(acc) * sa, sw, bias), act);
+  float v[1] = {fmaf(float(acc) * sa, sw, bias)};
+  activate<1>(v, act);
+  return v[0];
 }
 
 // CUDA cores (dp4a), any alignment: 64 x 64 tile, 64 of k a step, a 4 x 4
@@ -114,7 +128,7 @@ __device__ __forceinline__ void store4(const LinearArgs &p, const int4 acc, int6
                                        const float (&bias)[4], bool vec, bool real) {
   float v[4] = {fmaf(float(acc.x) * sa, sw[0], bias[0]), fmaf(float(acc.y) * sa, sw[1], bias[1]),
                 fmaf(float(acc.z) * sa, sw[2], bias[2]), fmaf(float(acc.w) * sa, sw[3], bias[3])};
-  apply_act_n<4>(v, p.act);
+  activate<4>(v, p.act);
   T *y = static_cast<T *>(p.y) + m * p.y_stride + n;
   if (vec) {
     struct alignas(4 * sizeof(T)) Four {
@@ -158,7 +172,7 @@ __device__ __forceinline__ void store_chunk(const LinearArgs &p, const CUtensorM
   float v[32];
 #pragma unroll
   for (int j = 0; j < COLS; ++j) v[j] = fmaf(float(int(acc[j])) * __shfl_sync(0xffffffffu, mine, j), sw, bias);
-  if (p.act != SPKV2_CUDA_ACT_NONE) apply_act32(v, p.act);
+  if (p.act != SPKV2_CUDA_ACT_NONE) activate<32>(v, p.act);
   if (COLS == 32 && p.y_tma) {
     if (n0 >= p.n) return;
     T *buf = buffers + (count & (BUFS - 1)) * 1024;

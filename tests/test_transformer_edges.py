@@ -77,3 +77,39 @@ def test_encoder_calls_behind_queued_work(gpu):
     torch.cuda.synchronize()
     assert torch.equal(a, want[0]) and torch.equal(b, want[1])
     encoder.close()
+
+
+# ------------------------------------------------------------------ product
+@gpu_test
+@pytest.mark.parametrize("activation", [None, "relu", "silu"])
+@pytest.mark.parametrize("m,k,n,pitch", [(1, 64, 64, 16), (2, 2048, 200, 16), (40, 512, 1000, 16), (5000, 256, 2048, 16),
+                                         (70, 333, 90, 1)])
+def test_product_keeps_what_is_not_finite(gpu, m, k, n, pitch, activation):
+    """A scale or bias of NaN shows in every element that it takes part in, whatever the activation, an
+    infinite one in the elements that the definition makes infinite or NaN, and nowhere else.  The sizes
+    reach one CTA a tile, clusters, pairs and the CUDA-core kernel."""
+    from spinnv2_b200 import transformer as T
+
+    g = gen(m + n)
+    a, w = codes_of(m, k, g, pitch), codes_of(n, k, g, pitch)
+    sa = torch.rand(m, generator=g, device="cuda") + 0.1
+    sw = (torch.rand(n, generator=g, device="cuda") + 0.1) / (5000 * math.sqrt(k))
+    bias = torch.randn(n, generator=g, device="cuda")
+    clean = {t: T.linear_i8(a, sa, w, sw, bias=bias, activation=activation, dtype=t) for t in TYPES}
+    rows, columns = torch.zeros(m, dtype=torch.bool, device="cuda"), torch.zeros(n, dtype=torch.bool, device="cuda")
+    rows[m // 2], columns[[0, n - 1, n // 3]] = True, True
+    sa[m // 2], sw[0], bias[n - 1], bias[n // 3] = math.nan, math.nan, math.nan, math.inf
+    v = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double() + bias.double()
+    want = torch.relu(v) if activation == "relu" else v * torch.sigmoid(v) if activation == "silu" else v
+    for dtype in TYPES:
+        got = T.linear_i8(a, sa, w, sw, bias=bias, activation=activation, dtype=dtype)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.isinf(got), torch.isinf(want))
+        keep = ~(rows[:, None] | columns)
+        assert torch.equal(got[keep], clean[dtype][keep])
+    bias[n // 3] = -math.inf
+    if activation == "relu":
+        got = T.linear_i8(a, sa, w, sw, bias=bias, activation=activation, dtype=torch.float32)
+        keep = torch.ones(m, dtype=torch.bool, device="cuda")
+        keep[m // 2] = False
+        assert not got[keep, n // 3].any()
