@@ -634,6 +634,8 @@ extern "C" int spkv2_cuda_linear_i8(const Spkv2LinearI8 *a, void *stream) {
 extern "C" int spkv2_cuda_transformer_status(int *code) {
   if (!code) return -1;
   *code = 0;
+  // Copies of the words alone would not wait for streams that do not block the default one.
+  if (const int rc = cuda_status(cudaDeviceSynchronize())) return rc;
   int (*const take[])(int *) = {linear_status, cross_tc_status, cross_step_status};
   int first = 0;
   for (auto t : take) {

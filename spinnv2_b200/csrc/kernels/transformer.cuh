@@ -88,7 +88,7 @@ inline int allow_smem(size_t bytes) {
 }
 
 // Reads and clears the status word (a device variable) of a file's kernels on
-// the current device; waits for the device's work.
+// the current device, whose work has ended.
 template <class Word>
 inline int take_status(Word &word, int *code) {
   *code = 0;

@@ -113,3 +113,24 @@ def test_product_keeps_what_is_not_finite(gpu, m, k, n, pitch, activation):
         keep = torch.ones(m, dtype=torch.bool, device="cuda")
         keep[m // 2] = False
         assert not got[keep, n // 3].any()
+
+
+@gpu_test
+def test_check_waits_for_every_stream(gpu):
+    """check() answers for all calls before it, on whatever stream."""
+    from spinnv2_b200 import transformer as T
+
+    side = torch.cuda.Stream()
+    matrix = torch.randn(8192, 8192, generator=gen(1), device="cuda")
+    q, k, v = inputs(2, 40, 300, 4, 2, 64, torch.bfloat16)
+    out, answer = torch.empty_like(matrix), torch.empty_like(q)
+    torch.mm(matrix, matrix, out=out)  # loaded: a first launch may wait for the device
+    T.cross_attention(q, k, v, out=answer)
+    T.check()
+    with torch.cuda.stream(side):
+        for _ in range(10):  # some 0.2 s
+            torch.mm(matrix, matrix, out=out)
+    T.cross_attention(q, k, v, out=answer, stream=side)
+    assert not side.query()
+    T.check()
+    assert side.query()
