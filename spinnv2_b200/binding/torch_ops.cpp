@@ -100,6 +100,11 @@ Rows rows_of(const at::Tensor &t, const char *name) {
   if (dims < 1) throw Bad{PyExc_ValueError, std::string(name) + ": expected [..., width], got a scalar"};
   Rows r;
   r.width = size[dims - 1];
+  if (t.numel() == 0) {  // no row is read or written, so its place does not matter
+    for (int64_t i = 0; i < dims - 1; ++i) r.rows *= size[i];
+    r.stride = r.width;
+    return r;
+  }
   for (int64_t i = dims - 2; i >= 0; --i) {
     if (size[i] == 1) continue;
     if (r.rows == 1)

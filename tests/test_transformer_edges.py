@@ -134,3 +134,42 @@ def test_check_waits_for_every_stream(gpu):
     assert not side.query()
     T.check()
     assert side.query()
+
+
+# ------------------------------------------------------------------ empty dimensions
+@gpu_test
+@pytest.mark.parametrize("shape", [(2, 0), (0, 2), (0, 0), (3, 0, 2), (0,), (2, 5, 0)])
+def test_nothing_to_write(gpu, shape):
+    """A call with an empty dimension, wherever it is, answers with an empty tensor of its shape."""
+    from spinnv2_b200 import transformer as T
+
+    for dtype in TYPES:
+        x = torch.zeros(*shape, 64, dtype=dtype, device="cuda")
+        w = torch.ones(64, dtype=dtype, device="cuda")
+        for residual in (None, x.clone()):
+            codes, scale, total = T.rms_norm_i8(x, w, residual)
+            assert codes.shape == total.shape == x.shape and scale.shape == shape and total.dtype is dtype
+        codes, scale = T.quantize_rows_i8(x)
+        assert codes.shape == x.shape and scale.shape == shape
+        assert T.dequantize_rows_i8(codes, scale, dtype).shape == x.shape
+        weight, ws = torch.zeros(48, 64, dtype=torch.int8, device="cuda"), torch.ones(48, device="cuda")
+        y = T.linear_i8(codes, scale, weight, ws, activation="relu", dtype=dtype)
+        assert y.shape == (*shape, 48) and y.dtype is dtype
+    given = torch.zeros(*shape, 64, dtype=torch.int8, device="cuda")
+    assert T.quantize_rows_i8(x, out=given)[0] is given
+
+
+@gpu_test
+def test_layer_of_no_tokens(gpu):
+    from spinnv2_b200.decoder import CrossAttentionLayer
+
+    layer = CrossAttentionLayer.random(256, 128, 4, 2, 64)
+    states = layer.states(torch.randn(2, 9, 128, device="cuda"))
+    x = torch.zeros(2, 0, 256, dtype=torch.bfloat16, device="cuda")
+    y, stream = layer.step(x, x.clone(), states)
+    assert y.shape == stream.shape == x.shape
+    y, _ = layer.step(x[:0], None, [t[:0] for t in states])
+    assert y.shape == (0, 0, 256)
+    none = layer.states(torch.zeros(2, 0, 128, device="cuda"))  # images of no positions
+    y, _ = layer.step(torch.ones(2, 3, 256, dtype=torch.bfloat16, device="cuda"), None, none)
+    assert y.shape == (2, 3, 256) and not y.any()
