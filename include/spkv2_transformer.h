@@ -89,7 +89,7 @@ typedef struct {
 
 int spkv2_cuda_quantize_rows_i8(const Spkv2QuantizeRowsI8 *args, void *stream);
 
-/* y = codes * scale[row]; up to 2^33 elements. */
+/* y = codes * scale[row]. */
 typedef struct {
     const int8_t *codes; /* [rows, width] */
     const float *scale;  /* [rows] */

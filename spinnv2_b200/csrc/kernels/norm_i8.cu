@@ -373,18 +373,40 @@ __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
   }
 }
 
-// VW codes a thread; chunks of all rows in one list.
+// The pieces of a matrix's rows in one list, a thread each: fn(row, piece of the row).
+// The list is counted in 32 bits, so it holds at most `most` rows at a time: all of
+// them, but for some 2^31 pieces and more.
+struct Pieces {
+  int64_t rows;
+  uint32_t most;
+  FastDiv per_row;
+  Pieces(int64_t n, int64_t each) : rows(n), most(uint32_t(std::min<int64_t>(n, INT32_MAX / each))), per_row(uint32_t(each)) {}
+  // 256 threads a block; several pieces a thread once all SMs are full (eight blocks each).
+  unsigned grid() const { return unsigned(std::min<int64_t>(ceil_div(int64_t(most) * per_row.d, 256), int64_t(sm_count()) * 64)); }
+};
+template <class F>
+__device__ __forceinline__ void for_pieces(const Pieces &p, F &&fn) {
+  for (int64_t row0 = 0; row0 < p.rows; row0 += p.most) {
+    const uint32_t count = uint32_t(min(int64_t(p.most), p.rows - row0)) * p.per_row.d;
+    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u) {
+      const uint32_t row = p.per_row.div(i);
+      fn(row0 + row, i - row * p.per_row.d);
+    }
+  }
+}
+
+// VW codes a thread.
 template <class T, int VW>
 __global__ void __launch_bounds__(256)
-    row_values_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, uint32_t chunks,
-                      FastDiv per_row, int64_t codes_stride, int64_t y_stride) {
+    row_values_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, Pieces pieces,
+                      int64_t codes_stride, int64_t y_stride) {
   pdl_launch_dependents();
   pdl_wait();
-  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < chunks; i += gridDim.x * 256u) {
-    const uint32_t row = per_row.div(i), c = (i - row * per_row.d) * VW;
+  for_pieces(pieces, [&](int64_t row, uint32_t piece) {
+    const uint32_t c = piece * VW;
     const float s = __ldg(scale + row);
-    const Vec<int8_t, VW> q = *reinterpret_cast<const Vec<int8_t, VW> *>(codes + int64_t(row) * codes_stride + c);
-    T *to = y + int64_t(row) * y_stride + c;
+    const Vec<int8_t, VW> q = *reinterpret_cast<const Vec<int8_t, VW> *>(codes + row * codes_stride + c);
+    T *to = y + row * y_stride + c;
     constexpr int S = VW * sizeof(T) > 16 ? 16 / sizeof(T) : VW;  // elements of a store
 #pragma unroll
     for (int k = 0; k < VW; k += S) {
@@ -393,7 +415,7 @@ __global__ void __launch_bounds__(256)
       for (int e = 0; e < S; ++e) o.v[e] = from_f32<T>(float(q.v[k + e]) * s);
       *reinterpret_cast<Vec<T, S> *>(to + k) = o;
     }
-  }
+  });
 }
 
 // The same where rows of y do not lie on 16-byte boundaries, or end inside one: a
@@ -402,17 +424,16 @@ __global__ void __launch_bounds__(256)
 template <class T>
 __global__ void __launch_bounds__(256)
     row_values_shifted_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scale, T *__restrict__ y, int width,
-                              uint32_t chunks, FastDiv per_row, int64_t codes_stride, int64_t y_stride, bool vec_codes) {
+                              Pieces pieces, int64_t codes_stride, int64_t y_stride, bool vec_codes) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int U = 16 / sizeof(T);
-  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < chunks; i += gridDim.x * 256u) {
-    const uint32_t row = per_row.div(i), k = i - row * per_row.d;
-    T *to = y + int64_t(row) * y_stride;
-    const int8_t *from = codes + int64_t(row) * codes_stride;
+  for_pieces(pieces, [&](int64_t row, uint32_t k) {
+    T *to = y + row * y_stride;
+    const int8_t *from = codes + row * codes_stride;
     const int head = int((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / int(sizeof(T));
     const int c = k == 0 ? 0 : head + int(k - 1) * U, end = min(k == 0 ? head : c + U, width);
-    if (c >= end) continue;
+    if (c >= end) return;
     const float s = __ldg(scale + row);
     if (k > 0 && c + U <= width) {
       Vec<T, U> o;
@@ -433,7 +454,7 @@ __global__ void __launch_bounds__(256)
     } else {
       for (int e = c; e < end; ++e) to[e] = from_f32<T>(float(from[e]) * s);
     }
-  }
+  });
 }
 
 template <class T, bool NORM, bool STAGED>
@@ -484,12 +505,9 @@ int launch_rows(const RowArgs &a, int32_t dtype, cudaStream_t s) {
 
 template <class T, int VW>
 int launch_values(const Spkv2DequantizeRowsI8 *a, cudaStream_t s) {
-  const int64_t per_row = a->width / VW, chunks = per_row * a->rows;
-  if (chunks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-  // Several chunks a thread once all SMs are full (eight blocks each).
-  const unsigned grid = unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64));
-  return cuda_status(launch_kernel(row_values_kernel<T, VW>, grid, 256u, 0, s, 1, a->codes, a->scale, static_cast<T *>(a->y),
-                                   uint32_t(chunks), FastDiv(uint32_t(per_row)), a->codes_stride, a->y_stride));
+  const Pieces pieces(a->rows, a->width / VW);
+  return cuda_status(launch_kernel(row_values_kernel<T, VW>, pieces.grid(), 256u, 0, s, 1, a->codes, a->scale, static_cast<T *>(a->y),
+                                   pieces, a->codes_stride, a->y_stride));
 }
 
 bool bad_extent(int64_t rows, int64_t width) { return rows < 0 || rows > INT32_MAX || width < 1 || width > kMaxWidth; }
@@ -541,12 +559,9 @@ extern "C" int spkv2_cuda_dequantize_rows_i8(const Spkv2DequantizeRowsI8 *a, voi
     const int vy = vector_width(16 / int(size), a->width, reinterpret_cast<uintptr_t>(a->y) / size, many ? a->y_stride : 0);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (std::min(vw, vy) < 16 / int(size)) {
-      const int64_t per_row = 1 + ceil_div(a->width, 16 / size), chunks = per_row * a->rows;
-      if (chunks > INT32_MAX) return SPKV2_ERR_UNSUPPORTED;
-      const unsigned grid = unsigned(std::min<int64_t>(ceil_div(chunks, 256), int64_t(sm_count()) * 64));
-      return cuda_status(launch_kernel(row_values_shifted_kernel<T>, grid, 256u, 0, s, 1, a->codes, a->scale,
-                                       static_cast<T *>(a->y), int(a->width), uint32_t(chunks), FastDiv(uint32_t(per_row)),
-                                       a->codes_stride, a->y_stride,
+      const Pieces pieces(a->rows, 1 + ceil_div(a->width, 16 / size));
+      return cuda_status(launch_kernel(row_values_shifted_kernel<T>, pieces.grid(), 256u, 0, s, 1, a->codes, a->scale,
+                                       static_cast<T *>(a->y), int(a->width), pieces, a->codes_stride, a->y_stride,
                                        reinterpret_cast<uintptr_t>(a->codes) % 4 == 0 && (!many || a->codes_stride % 4 == 0)));
     }
     if (vw == 16) return launch_values<T, 16>(a, s);

@@ -173,3 +173,21 @@ def test_layer_of_no_tokens(gpu):
     none = layer.states(torch.zeros(2, 0, 128, device="cuda"))  # images of no positions
     y, _ = layer.step(torch.ones(2, 3, 256, dtype=torch.bfloat16, device="cuda"), None, none)
     assert y.shape == (2, 3, 256) and not y.any()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_values_of_very_many_rows(gpu, dtype):
+    """As many rows as an extent can have, of one code each: more pieces than 32 bits count."""
+    from spinnv2_b200 import transformer as T
+
+    rows = 2**30 + 11
+    codes = torch.zeros(rows, 1, dtype=torch.int8, device="cuda")
+    scale = torch.full((rows,), 0.5, device="cuda")
+    ends = [slice(0, 1000), slice(2**29 - 500, 2**29 + 500), slice(rows - 1000, rows)]
+    for i, at in enumerate(ends):
+        codes[at, 0] = torch.randint(-127, 128, (1000,), generator=gen(i), device="cuda").to(torch.int8)
+    got = T.dequantize_rows_i8(codes, scale, dtype)
+    for at in ends:
+        assert torch.equal(got[at], (codes[at].float() * 0.5).to(dtype))
+    assert int(torch.count_nonzero(got)) == int(torch.count_nonzero(codes))
