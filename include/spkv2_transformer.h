@@ -56,9 +56,11 @@ extern "C" {
 
 /* s = x + residual;  y = s * weight / sqrt(mean(s^2) + eps);
  * scale = max|y| / 127;  codes = round_half_even(y / scale), per row.
- * A row of zeros has scale 0 and codes 0; a row that holds an infinity or a
- * NaN has scale NaN and codes 0.  sum (if given) receives s in x's type and
- * may be x or residual itself.  width: 1 .. 2^24. */
+ * A row of zeros has scale 0 and codes 0; a row whose s (an fp32 sum) or
+ * weight holds an infinity or a NaN has scale NaN and codes 0.  Finite rows may
+ * lie anywhere in fp32's range, squares beyond it included; weights other than
+ * 0 from 2^-64 to 2^64.  sum (if given) receives s in x's type and may be x or
+ * residual itself.  width: 1 .. 2^24. */
 typedef struct {
     const void *x;        /* [rows, width] */
     const void *residual; /* [rows, width] in x's type, or NULL */

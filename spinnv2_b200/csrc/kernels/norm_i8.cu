@@ -106,6 +106,27 @@ __device__ __forceinline__ uint4 contract(const float (&f)[8], __half) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Values of a row whose sum of squares may leave fp32's range, or lose bits at its
+// lower end, are taken as s / 2^x instead, x the exponent of the largest |s| among
+// them: no square of those overflows, nor a product with a weight, and what
+// underflows is too small to matter.  Inside the range |s| < 2^30.
+__device__ __forceinline__ bool out_of_range(float ss) { return !(ss >= 0x1p-90f && ss <= 0x1p60f); }
+__device__ __forceinline__ int exponent_of(float top) { return ilogbf(top) + 1; }
+// 2^n for |n| up to 298 as two factors.
+struct TwoTo {
+  float a, b;
+  __device__ __forceinline__ explicit TwoTo(int n) : a(scalbnf(1.0f, n / 2)), b(scalbnf(1.0f, n - n / 2)) {}
+  __device__ __forceinline__ float of(float v) const { return v * a * b; }
+};
+
+// The scale of a row whose ss and amax are of s / 2^x.
+__device__ __noinline__ float scale_from(float ss, float amax, int x, int64_t width, float eps) {
+  if (!(amax < INFINITY)) return __uint_as_float(0x7fc00000u);
+  if (amax == 0.0f) return 0.0f;
+  const double mean = scalbn(double(ss) / double(width), 2 * x) + double(eps);
+  return float(scalbn(double(amax), x) / sqrt(mean) / 127.0);
+}
+
 // A row's scale (its first thread writes it) and the factor of its codes.
 template <bool NORM>
 __device__ __forceinline__ CodeScale finish_row(const RowArgs &p, int64_t row, float ss, float amax, bool &finite, bool writes) {
@@ -119,6 +140,17 @@ __device__ __forceinline__ CodeScale finish_row(const RowArgs &p, int64_t row, f
 
 __host__ __device__ __forceinline__ int stage_at(int e, int u) { return e + e / u; }
 __host__ __device__ __forceinline__ int stage_floats(int width, int u) { return stage_at((width + u - 1) / u * u, u); }
+
+// The threads of one row of a block; at most two rows of a block have several warps.
+// (The barrier's number is a constant: one in a register reserves all sixteen, and
+// fewer blocks fit an SM.)
+__device__ __forceinline__ void row_barrier(int row, int threads) {
+  if (row == 0)
+    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+  else
+    asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+}
+constexpr int kNoValues = -1024, kShift = 1024;  // exponent of a thread that has only zeros; makes exponents positive
 
 // Bound by memory: every element is read once, kept in registers (16 a thread)
 // through the row's two reductions, and its code written once.  A block for each
@@ -195,11 +227,23 @@ __global__ void __launch_bounds__(1024)
     xv[i] = in ? *reinterpret_cast<const uint4 *>(x + head + k * U) : none;
     if (NORM && p.residual) rv[i] = in ? *reinterpret_cast<const uint4 *>(r + head + k * U) : none;
   }
-  if (NORM) {
+  // Held from here on, the weights would cost staged fp32 rows spills (9000 x 2647: 74
+  // us, read where they are used 62).
+  constexpr bool HOLDS = NORM && !(STAGED && sizeof(T) == 4);
+  auto unit_weights = [&](int i) { return (t + i * tpr) * U < width ? weights((t + i * tpr) * U) : none; };
+  if (HOLDS) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) wv[i] = (t + i * tpr) * U < width ? weights((t + i * tpr) * U) : none;
+    for (int i = 0; i < N; ++i) wv[i] = unit_weights(i);
   }
   float v[N][U];
+  auto unstage = [&] {  // this thread's units; zeros past the width
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (t + i * tpr) * U;
+#pragma unroll
+      for (int e = 0; e < U; ++e) v[i][e] = real && c < width ? mine[(t + i * tpr) * (U + 1) + e] : 0.0f;
+    }
+  };
   if (STAGED) {
     // Places of a unit's elements: element head + k U + e lies at k (U + 1) + place[e].
     int place[U];
@@ -238,12 +282,7 @@ __global__ void __launch_bounds__(1024)
       if (t < (width + U - 1) / U * U - width) mine[stage_at(width + t, U)] = 0.0f;
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (t + i * tpr) * U;
-#pragma unroll
-      for (int e = 0; e < U; ++e) v[i][e] = real && c < width ? mine[(t + i * tpr) * (U + 1) + e] : 0.0f;
-    }
+    unstage();
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -259,42 +298,112 @@ __global__ void __launch_bounds__(1024)
     }
   }
   float ss = 0.0f, mx = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {  // units past the width hold zeros
+  auto weigh = [&](const uint4 &raw, float (&f)[U]) {  // a unit's products
     if (NORM) {
       float wf[U];
-      expand(wv[i], wf, T{});
+      expand(raw, wf, T{});
 #pragma unroll
-      for (int e = 0; e < U; ++e) {
-        ss = fmaf(v[i][e], v[i][e], ss);
-        v[i][e] *= wf[e];
-      }
+      for (int e = 0; e < U; ++e) f[e] *= wf[e];
     }
 #pragma unroll
-    for (int e = 0; e < U; ++e) mx = max_nan(mx, fabsf(v[i][e]));
+    for (int e = 0; e < U; ++e) mx = max_nan(mx, fabsf(f[e]));
+  };
+  // A thread whose values leave the range scales its own; an infinite ss says so to the
+  // others of the row, who follow below.  It needs s once more: staged rows have it in
+  // shared memory, the others form their products after the test.
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (NORM) {
+#pragma unroll
+      for (int e = 0; e < U; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+    }
+    if (!NORM || STAGED) weigh(NORM && !HOLDS ? unit_weights(i) : wv[i], v[i]);
   }
-  for (int o = min(tpr, 32) / 2; o; o >>= 1) {
-    if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  int x_exp = 0;
+  float own = ss;
+  if (NORM && out_of_range(ss)) {
+    if (STAGED) unstage();
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < U; ++e) top = max_nan(top, fabsf(v[i][e]));
+    own = 0.0f;
+    if (top > 0.0f && top < INFINITY) {
+      x_exp = exponent_of(top);
+      const TwoTo down(-x_exp);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+          v[i][e] = down.of(v[i][e]);
+          own = fmaf(v[i][e], v[i][e], own);
+        }
+      ss = INFINITY;
+    } else if (top == 0.0f) {
+      x_exp = kNoValues;
+    } else {
+      ss = 0.0f;
+    }
+    mx = top < INFINITY ? 0.0f : __uint_as_float(0x7fc00000u);
+    if (STAGED) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) weigh(unit_weights(i), v[i]);
+    }
   }
-  if (wpr > 1) {
+  if (NORM && !STAGED) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) weigh(wv[i], v[i]);
+  }
+  auto join = [&](float &sum, float &top, bool again) {
+    for (int o = min(tpr, 32) / 2; o; o >>= 1) {
+      if (NORM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (wpr <= 1) return;
+    if (again) row_barrier(sub, tpr);  // the sums before have been read
     if (lane == 0) {
-      s_sum[warp] = ss;
-      s_max[warp] = mx;
+      s_sum[warp] = sum;
+      s_max[warp] = top;
     }
-    __syncthreads();
+    if (again)
+      row_barrier(sub, tpr);
+    else
+      __syncthreads();
     const int w0 = sub * wpr;
-    ss = lane < wpr ? s_sum[w0 + lane] : 0.0f;
-    mx = lane < wpr ? s_max[w0 + lane] : 0.0f;
+    sum = lane < wpr ? s_sum[w0 + lane] : 0.0f;
+    top = lane < wpr ? s_max[w0 + lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-      if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (NORM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  };
+  float amax = mx;
+  join(ss, amax, false);
+  bool scaled = false;
+  if (NORM) {
+    scaled = ss == INFINITY;
+    if (__any_sync(0xffffffffu, scaled)) {  // the warps of one row, or rows that share a warp
+      float unused = 0.0f, row_exp = float(x_exp + kShift);  // not below 0, where the maximum starts
+      join(unused, row_exp, true);
+      const TwoTo down(x_exp + kShift - int(row_exp));
+      float row_ss = down.of(down.of(own)), row_max = down.of(mx);
+      join(row_ss, row_max, true);
+      if (scaled) {
+        ss = row_ss, amax = row_max;
+        x_exp = int(row_exp) - kShift;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < U; ++e) v[i][e] = down.of(v[i][e]);
+      }
     }
   }
   if (!real) return;
   bool finite;
-  const CodeScale cs = finish_row<NORM>(p, row, ss, mx, finite, t == 0);
+  const CodeScale cs = finish_row<NORM>(p, row, ss, amax, finite, t == 0 && !scaled);
+  if (NORM && scaled && t == 0) p.scale[row] = scale_from(ss, amax, x_exp, p.width, p.eps);
   int8_t *codes = p.codes + row * p.codes_stride;
   if (cs.pre != 1.0f || !finite) {
 #pragma unroll
@@ -321,28 +430,9 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// Rows wider than kMostWidth, the registers of a block: one block a row, which is read twice, the second time from L2; the sum is written in the
-// second pass, as it may take x's or the residual's place.
-template <class T, bool NORM>
-__global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ float s_sum[32];
-  __shared__ float s_max[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const int64_t row = blockIdx.x;
-  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
-  const T *r = NORM && p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
-  const T *w = static_cast<const T *>(p.weight);
-  float ss = 0.0f;
-  float mx = 0.0f;
-#pragma unroll 4
-  for (int64_t i = tid; i < p.width; i += threads) {
-    float s = to_f32(x[i]);
-    if (r) s += to_f32(r[i]);
-    ss = fmaf(s, s, ss);
-    mx = max_nan(mx, fabsf(NORM ? s * to_f32(w[i]) : s));
-  }
+// A block's sums and maxima, joined for all of its threads.
+__device__ __forceinline__ void join_block(float &ss, float &mx, float *s_sum, float *s_max) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -359,6 +449,70 @@ __global__ void __launch_bounds__(1024) wide_codes_kernel(RowArgs p) {
   for (int o = 16; o; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
     mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+}
+
+// A wide row whose sums left the range: all of it again, from s / 2^x.
+template <class T>
+__device__ __noinline__ void wide_row_scaled(RowArgs p, int64_t row, float *s_sum, float *s_max) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+  const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
+  const T *w = static_cast<const T *>(p.weight);
+  auto value = [&](int64_t i) { return r ? to_f32(x[i]) + to_f32(r[i]) : to_f32(x[i]); };
+  float ss = 0.0f, mx = 0.0f;
+  for (int64_t i = tid; i < p.width; i += threads) mx = max_nan(mx, fabsf(value(i)));
+  __syncthreads();  // the sums before have been read
+  join_block(ss, mx, s_sum, s_max);
+  const int x_exp = mx > 0.0f && mx < INFINITY ? exponent_of(mx) : 0;
+  if (mx < INFINITY) {
+    ss = mx = 0.0f;
+    for (int64_t i = tid; i < p.width; i += threads) {
+      const float s = scalbnf(value(i), -x_exp);
+      ss = fmaf(s, s, ss);
+      mx = max_nan(mx, fabsf(s * to_f32(w[i])));
+    }
+    __syncthreads();
+    join_block(ss, mx, s_sum, s_max);
+  }
+  if (tid == 0) p.scale[row] = scale_from(ss, mx, x_exp, p.width, p.eps);
+  const bool finite = mx < INFINITY;
+  const CodeScale c = code_scale(finite ? mx : 0.0f);
+  T *sum = p.sum ? static_cast<T *>(p.sum) + row * p.sum_stride : nullptr;
+  int8_t *codes = p.codes + row * p.codes_stride;
+  for (int64_t i = tid; i < p.width; i += threads) {
+    const float s = value(i);
+    codes[i] = finite ? int8_t(code_bits(scalbnf(s, -x_exp) * to_f32(w[i]) * c.pre, c.inv)) : int8_t(0);
+    if (sum) sum[i] = from_f32<T>(s);
+  }
+}
+
+// Rows wider than kMostWidth, the registers of a block: one block a row, which is read twice, the second time from L2; the sum is written in the
+// second pass, as it may take x's or the residual's place.
+template <class T, bool NORM>
+__global__ void __launch_bounds__(1024, 2) wide_codes_kernel(RowArgs p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ float s_sum[32];
+  __shared__ float s_max[32];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int64_t row = blockIdx.x;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+  const T *r = NORM && p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
+  const T *w = static_cast<const T *>(p.weight);
+  float ss = 0.0f;
+  float mx = 0.0f;
+#pragma unroll 4
+  for (int64_t i = tid; i < p.width; i += threads) {
+    float s = to_f32(x[i]);
+    if (r) s += to_f32(r[i]);
+    ss = fmaf(s, s, ss);
+    mx = max_nan(mx, fabsf(NORM ? s * to_f32(w[i]) : s));
+  }
+  join_block(ss, mx, s_sum, s_max);
+  if (NORM && out_of_range(ss)) {
+    wide_row_scaled<T>(p, row, s_sum, s_max);
+    return;
   }
   bool finite;
   const CodeScale c = finish_row<NORM>(p, row, ss, mx, finite, tid == 0);

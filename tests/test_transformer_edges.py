@@ -191,3 +191,52 @@ def test_values_of_very_many_rows(gpu, dtype):
     for at in ends:
         assert torch.equal(got[at], (codes[at].float() * 0.5).to(dtype))
     assert int(torch.count_nonzero(got)) == int(torch.count_nonzero(codes))
+
+
+# ------------------------------------------------------------------ norm and codes
+# Widths: a unit of 16 bytes, rows that share a warp, rows of two warps that share a block, rows of many warps,
+# rows read twice; each also where rows do not lie on 16-byte boundaries.
+@gpu_test
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [3, 8, 64, 100, 250, 1000, 1024, 2048, 5001, 16384, 40000])
+def test_norm_of_rows_of_any_size(gpu, width, dtype):
+    """The scale of every finite row is what the definition gives, also where the squares of its values leave
+    fp32's range, or their products with the weights do.  The products are formed after the row was scaled by a
+    power of two, so the bounds are those of ordinary rows."""
+    from spinnv2_b200 import transformer as T
+
+    info = torch.finfo(dtype)
+    g = gen(width)
+    x = torch.randn(14, width, generator=g, device="cuda", dtype=torch.float64)
+    low = info.smallest_normal * 2.0**-8 if dtype is not torch.float32 else info.smallest_normal
+    sizes = [1.0, info.max / 64, 1e4, info.max / 2**40, info.max**0.5, info.tiny**0.5, 2**-12, low * 64, info.tiny * 2**30, 0.0]
+    for i, size in enumerate(sizes):
+        x[i] *= min(size, info.max / 64)
+    x[10] = 0
+    x[10, width - 1] = info.smallest_normal  # one small value
+    x[11, width // 2] = info.max  # one huge value beside ordinary ones
+    x[12] *= info.tiny
+    x[12, 0] = 1.0  # one ordinary value beside tiny ones
+    x[13] = info.max
+    x = x.to(dtype)
+    assert torch.isfinite(x).all()
+    r = (0.5 * torch.randn(x.shape, generator=g, device="cuda").double() * x.double()).to(dtype)
+    r = torch.where(torch.isfinite(x.float() + r.float()), r, 0)
+    ordinary = (1 + 0.2 * torch.randn(width, generator=g, device="cuda")).to(dtype)
+    wide = ordinary.clone()
+    if width > 3 and dtype is not torch.float16:
+        wide[1], wide[2] = 1e30, 1e-30
+    for weight in (ordinary, wide):
+        for eps in (0.0, 1e-6):
+            for residual in (None, r):
+                s = x.double() if residual is None else (x.float() + residual.float()).double()
+                mean = s.square().mean(-1, keepdim=True) + eps
+                y = torch.where(mean > 0, s * weight.double() / mean.sqrt(), 0.0)
+                top = y.abs().amax(-1)
+                assert torch.isfinite(top).all() and float(top.max()) < 1e38
+                codes, scale, _ = T.rms_norm_i8(x, weight, residual, eps=eps)
+                check_codes(codes, scale, y, width)
+                far = torch.zeros(14, width + 1, dtype=dtype, device="cuda")[:, 1:]  # rows off their boundaries
+                far.copy_(x)
+                again = T.rms_norm_i8(far, weight, residual, eps=eps)
+                assert torch.equal(again[0], codes) and torch.equal(again[1], scale)
