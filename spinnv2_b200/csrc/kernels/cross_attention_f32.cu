@@ -16,6 +16,11 @@
 // scores.  The scores' accumulators are the next product's A operand: its columns
 // t and t + 4 stand for keys 2 t and 2 t + 1 of eight, in both operands.
 //
+// An infinite value has no low part (inf - inf), and one next to the largest has an
+// infinite high part, so their products, though defined, come out as NaN.  Where such
+// values count, rows with an answer that is not finite are taken again by plain fp32
+// products.
+//
 // With too few row tiles for the SMs the CTAs of a cluster divide the keys, as in
 // the other kernels.  Bound by the MMAs and what splits their operands: 40 TFLOP/s of
 // answers (4 x 1024 x 16 heads, 1024 keys, width 128: 852 us; on CUDA cores 1339 us),
@@ -85,16 +90,63 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t b
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
+// A value whose high part is infinite.
+__device__ __forceinline__ bool unsplittable(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return u >= 0x7f7ff000u && u <= 0x7f800000u;
+}
+
+// One row by plain fp32 products, by a warp: `q` in shared memory, `mask` of its entry
+// or null, `out` its place.  Keys pass twice, once for m and l and once for the answer,
+// so that no sum is larger than the values that it weighs.
+template <int D>
+__device__ __noinline__ void plain_row(const float *q, const float *k, const float *v, float *out, int64_t k_stride, int64_t v_stride,
+                                       const uint8_t *mask, int keys, int width, float scale_log2) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  auto counts = [&](int j) { return !mask || mask[j] != 0; };
+  auto score = [&](int j) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < width) s = fmaf(q[lane + 32 * i], k[j * k_stride + lane + 32 * i], s);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    return s * scale_log2;
+  };
+  float m = -INFINITY, l = 0.0f;
+  for (int j = 0; j < keys; ++j) {
+    if (!counts(j)) continue;
+    const float s = score(j), top = fmaxf(m, s), use = top == -INFINITY ? 0.0f : top;
+    l = l * exp2f(m - use) + exp2f(s - use);
+    m = top;
+  }
+  const float use = m == -INFINITY ? 0.0f : m;
+  float o[N] = {};
+  for (int j = 0; j < keys; ++j) {
+    if (!counts(j)) continue;
+    const float p = exp2f(score(j) - use) / l;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < width) o[i] = fmaf(p, v[j * v_stride + lane + 32 * i], o[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (lane + 32 * i < width) out[lane + 32 * i] = l != 0.0f ? o[i] : 0.0f;
+}
+
 template <int D, int W>
 __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross_f32_kernel(AttnArgs a, int csize, bool vec, bool vec_q, bool vec_out) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using S = F32Smem<D, W>;
   S &sm = *reinterpret_cast<S *>(smem_raw);
+  __shared__ uint32_t s_again[2];  // rows of the CTA with an answer that is not finite
   constexpr int KW = 64 / W, NT = KW / 8;  // keys of a warp in a tile, in eights
   constexpr int G = NT < 4 ? NT : 4;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid < 2) s_again[tid] = 0;
   const int rank = csize > 1 ? int(cluster_rank()) : 0;
   int item = int(blockIdx.x) / csize;
   const int r0 = item % a.row_tiles * S::rows;
@@ -261,17 +313,38 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
   }
   auto out_row = [&](int row) { return static_cast<float *>(a.out) + b * a.os[0] + row_offset(a, a.os, hk, row); };
+  // Rows with an answer that is not finite, once more where a value that counts cannot be
+  // split.  A NaN among the keys is in every answer, and leaves nothing to mend.
+  auto mend = [&] {
+    if (!(s_again[0] | s_again[1])) return;
+    const uint8_t *mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+    bool found = false, nan = false;
+    for (int e = tid; e < S::rows * D; e += kThreads) found |= unsplittable(sm.q[e / D][e % D]);
+    for (int j = warp; j < keys; j += kThreads / 32) {
+      if (mask && mask[j] == 0) continue;
+      for (int c = lane; c < a.width; c += 32) {
+        const float x = k[j * a.ks[1] + c];
+        found |= unsplittable(x) || unsplittable(v[j * a.vs[1] + c]);
+        nan |= x != x;
+      }
+    }
+    if (!__syncthreads_or(found) || __syncthreads_or(nan)) return;
+    for (int r = warp; r < S::rows; r += kThreads / 32)
+      if ((s_again[r >> 5] >> (r & 31)) & 1)
+        plain_row<D>(sm.q[r], k, v, out_row(r0 + r), a.ks[1], a.vs[1], mask, keys, a.width, a.scale_log2);
+  };
   if (W == 1 && csize == 1) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = r0 + qr + h * 8 + g;
       if (row >= a.rows) continue;
       const float inv = l[h] != 0.0f ? 1.0f / l[h] : 0.0f;
-      float *out = out_row(row);
+      float *out = out_row(row), size[4] = {};  // sums that are finite only if all answers are
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
         const int c = n * 8 + 2 * t;
         const float x = o[n][2 * h] * inv, y = o[n][2 * h + 1] * inv;
+        size[n & 3] += fabsf(x) + fabsf(y);
         if (vec_out) {
           if (c < a.width) *reinterpret_cast<float2 *>(out + c) = make_float2(x, y);
         } else {
@@ -279,9 +352,17 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
           if (c + 1 < a.width) out[c + 1] = y;
         }
       }
+      if (!(size[0] + size[1] + size[2] + size[3] < INFINITY)) atomicOr(&s_again[(qr + h * 8 + g) >> 5], 1u << ((qr + h * 8 + g) & 31));
     }
+    __syncthreads();
+    mend();
     return;
   }
+  auto put = [&](int r, int c, float x) {
+    if (c >= a.width) return;
+    out_row(r0 + r)[c] = x;
+    if (!(fabsf(x) < INFINITY)) atomicOr(&s_again[r >> 5], 1u << (r & 31));
+  };
   __syncthreads();  // the last values have been read: O goes over keys and values
   float *part = &sm.k[0][0];
 #pragma unroll
@@ -314,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
         sum = fmaf(sm.l[at + w * 16], f, sum);
       }
       if (csize == 1) {
-        if (c < a.width) out_row(r0 + r)[c] = sum != 0.0f ? acc / sum : 0.0f;
+        put(r, c, sum != 0.0f ? acc / sum : 0.0f);
       } else {
         part[at * D + c] = acc;
         if (c == 0) {
@@ -346,11 +427,14 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : W == 4 ? 4 : 3) cross
         acc = fmaf(ok[n], f, acc);
         sum = fmaf(lk[n], f, sum);
       }
-      if (c < a.width) out_row(r0 + r)[c] = sum != 0.0f ? acc / sum : 0.0f;
+      put(r, c, sum != 0.0f ? acc / sum : 0.0f);
     }
     __syncwarp();
-    cluster_sync();  // the peers have read this CTA's sums
+    cluster_sync();  // the peers have read this CTA's sums, and every answer is written
+  } else {
+    __syncthreads();
   }
+  mend();  // two CTAs of a cluster may mend one row; they write the same bits
 }
 
 template <int D, int W>

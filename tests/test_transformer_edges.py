@@ -240,3 +240,53 @@ def test_norm_of_rows_of_any_size(gpu, width, dtype):
                 far.copy_(x)
                 again = T.rms_norm_i8(far, weight, residual, eps=eps)
                 assert torch.equal(again[0], codes) and torch.equal(again[1], scale)
+
+
+@gpu_test
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d", [(1, 1, 200, 2, 2, 64), (2, 5, 70, 4, 2, 32), (1, 40, 300, 4, 2, 128),
+                                             (8, 130, 130, 16, 16, 40), (1, 33, 1500, 2, 1, 64), (2, 3, 40, 2, 2, 7)])
+def test_fp32_attention_with_values_at_the_end_of_the_type(gpu, b, lq, lk, hq, hk, d):
+    """Infinities and values next to the largest one, in keys and values that count: an answer is infinite, NaN
+    or finite as the definition says."""
+    from spinnv2_b200 import transformer as T
+
+    q, k, v = inputs(b, lq, lk, hq, hk, d, torch.float32, 31)
+    q, k = q * 0.2, k * 0.2  # no probability underflows
+    big = torch.finfo(torch.float32).max
+    group = hq // hk
+    for junk in (math.inf, -math.inf, big, -big):
+        vv = v.clone()
+        vv[0, lk // 2, hk - 1, d - 1] = junk
+        got = T.cross_attention(q, k, vv)
+        want, size, score = attention64(q, k, vv, None, 1 / math.sqrt(d))
+        clean = T.cross_attention(q, k, v)
+        other = torch.ones_like(got, dtype=torch.bool)
+        other[0, :, hq - group:] = False
+        assert torch.equal(got[other], clean[other])  # of other entries and heads
+        if math.isinf(junk):
+            hit = torch.zeros_like(other)
+            hit[0, :, hq - group:, d - 1] = True
+            assert (got[hit] == junk).all()
+            want, size, _ = attention64(q, k, v, None, 1 / math.sqrt(d))
+            got = torch.where(hit, want.float(), got)
+        tol = (lk + 64) * 8 * F32 * size + 2 * ((d + 16) * 4 * F32 * score + 64 * F32) * size
+        assert ((got.double() - want).abs() <= tol).all()
+    # A key of -infinity where the query is positive has no weight; one of +infinity leaves no number.
+    q[..., 0] = q[..., 0].abs() + 0.1
+    clean = T.cross_attention(q, k, v)
+    other = torch.ones_like(clean, dtype=torch.bool)
+    other[0, :, :group] = False
+    valid = torch.ones(b, lk, dtype=torch.bool, device="cuda")
+    valid[0, lk // 3] = False
+    want, size, score = (t[0, :, :group] for t in attention64(q, k, v, valid, 1 / math.sqrt(d)))
+    for junk in (math.inf, -math.inf):
+        kk = k.clone()
+        kk[0, lk // 3, 0, 0] = junk
+        got = T.cross_attention(q, kk, v)
+        assert torch.equal(got[other], clean[other])
+        got = got[0, :, :group]
+        if junk > 0:
+            assert torch.isnan(got).all()
+        else:
+            tol = (lk + 64) * 8 * F32 * size + 2 * ((d + 16) * 4 * F32 * score + 64 * F32) * size
+            assert ((got.double() - want).abs() <= tol).all()
