@@ -6,7 +6,8 @@ runtime, so the library needs nothing but the NVIDIA driver at load time.
 build_binding() compiles the torch binding of the decoder-layer operators
 beside it (_lib/_torch_ops.so), with g++ against the installed torch.
 Objects are rebuilt when a source or any header under csrc/ or include/
-is newer than the object.
+is newer than the object, the binding also when it was compiled for another
+torch or interpreter.
 """
 
 from __future__ import annotations
@@ -28,6 +29,7 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libspkv2_runtime.so"
 BINDING_SOURCE = PKG_DIR / "binding" / "torch_ops.cpp"
 BINDING_PATH = LIB_DIR / "_torch_ops.so"
+BINDING_STAMP = LIB_DIR / "_torch_ops.for"  # the torch and interpreter that it was compiled for
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = [
@@ -101,11 +103,15 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
 def build_binding(verbose: bool = False) -> Path:
     """Compile the torch binding of the decoder-layer operators (a CPython module for the
     interpreter and the torch that run this)."""
+    import torch
+
+    target = f"torch {torch.__version__}, {sys.implementation.cache_tag}\n"
+    if (BINDING_PATH.exists() and BINDING_STAMP.exists() and BINDING_STAMP.read_text() == target
+            and BINDING_PATH.stat().st_mtime >= max(
+                p.stat().st_mtime for p in (BINDING_SOURCE, INCLUDE / "spkv2_transformer.h"))):
+        return BINDING_PATH
     from torch.utils.cpp_extension import include_paths, library_paths
 
-    if BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= max(
-            p.stat().st_mtime for p in (BINDING_SOURCE, INCLUDE / "spkv2_transformer.h")):
-        return BINDING_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     includes = [INCLUDE, sysconfig.get_path("include"), Path(_nvcc()).parent.parent / "include", *include_paths()]
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(f"-I{p}" for p in includes),
@@ -116,6 +122,7 @@ def build_binding(verbose: bool = False) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING_SOURCE.name}:\n{res.stdout}\n{res.stderr}")
+    BINDING_STAMP.write_text(target)
     return BINDING_PATH
 
 

@@ -290,3 +290,41 @@ def test_fp32_attention_with_values_at_the_end_of_the_type(gpu, b, lq, lk, hq, h
         else:
             tol = (lk + 64) * 8 * F32 * size + 2 * ((d + 16) * 4 * F32 * score + 64 * F32) * size
             assert ((got.double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------ build
+def test_binding_is_built_for_the_torch_that_is_there(built, monkeypatch, tmp_path):
+    """The binding is compiled again for another torch or interpreter, and not otherwise."""
+    from spinnv2_b200.csrc import build as b
+
+    calls = []
+
+    def compiler(cmd, **_):
+        calls.append(cmd)
+        (tmp_path / "ops.so").write_text("")
+        return b.subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(b, "BINDING_PATH", tmp_path / "ops.so")
+    monkeypatch.setattr(b, "BINDING_STAMP", tmp_path / "ops.for")
+    monkeypatch.setattr(b.subprocess, "run", compiler)
+    for _ in range(2):
+        assert b.build_binding() == tmp_path / "ops.so" and len(calls) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    b.build_binding()
+    assert len(calls) == 2
+    b.build_binding()
+    assert len(calls) == 2
+    monkeypatch.setattr(b.sys.implementation, "cache_tag", "cpython-1")
+    b.build_binding()
+    assert len(calls) == 3
+
+
+def test_build_without_torch(built, monkeypatch, capsys):
+    """build() compiles the graph runtime where torch is not installed, and says what it left out."""
+    import sys
+
+    import __graft_entry__
+
+    monkeypatch.setitem(sys.modules, "torch", None)
+    __graft_entry__.build()
+    assert "torch is not installed" in capsys.readouterr().out
