@@ -328,3 +328,70 @@ def test_build_without_torch(built, monkeypatch, capsys):
     monkeypatch.setitem(sys.modules, "torch", None)
     __graft_entry__.build()
     assert "torch is not installed" in capsys.readouterr().out
+
+
+# ------------------------------------------------------------------ sizes past 32 bits, threads
+@gpu_test
+def test_product_of_more_than_2_to_31_answers(gpu):
+    from spinnv2_b200 import transformer as T
+
+    m, k, n = 70001, 64, 32768
+    g = gen(3)
+    a, w = codes_of(m, k, g), codes_of(n, k, g)
+    sa, sw = torch.rand(m, generator=g, device="cuda") + 0.1, torch.rand(n, generator=g, device="cuda") / 10000
+    y = T.linear_i8(a, sa, w, sw)
+    for at in (slice(0, 200), slice(65436, 65636), slice(m - 200, m)):  # 2^31 answers end at row 65536
+        exact = (a[at].double() @ w.double().t()) * sa[at, None].double() * sw.double()
+        assert ((y[at].double() - exact).abs() <= (U[y.dtype] + 4 * F32) * exact.abs()).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("offset", [0, 1])
+def test_rows_of_more_than_2_to_31_values(gpu, offset):
+    from spinnv2_b200 import transformer as T
+
+    rows, width = 2**19 + 137, 4096
+    ends = [slice(0, 50), slice(2**19 - 25, 2**19 + 25), slice(rows - 50, rows)]  # 2^31 values end at row 2^19
+    flat = torch.zeros(rows * width + offset, dtype=torch.bfloat16, device="cuda")
+    x = flat[offset:].view(rows, width)
+    w = (1 + 0.2 * torch.randn(width, generator=gen(1), device="cuda")).bfloat16()
+    for i, at in enumerate(ends):
+        x[at] = torch.randn(50, width, generator=gen(i + 2), device="cuda").bfloat16()
+    keep = [x[at].clone() for at in ends]
+    codes, scale, total = T.rms_norm_i8(x, w, x, sum_out=x)
+    assert total is x
+    values = T.dequantize_rows_i8(codes, scale)
+    for at, part in zip(ends, keep):
+        s = 2 * part.double()
+        y = s * w.double() / (s.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+        check_codes(codes[at], scale[at], y, width)
+        assert torch.equal(x[at], 2 * part)
+        assert torch.equal(values[at], (codes[at].float() * scale[at, None]).bfloat16())
+    assert int(torch.count_nonzero(scale)) == 150
+
+
+@gpu_test
+def test_calls_from_two_threads(gpu):
+    """Calls from two threads, each on a stream of its own, answer as they do one after another."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from spinnv2_b200 import transformer as T
+
+    def call(seed):
+        x = torch.randn(60, 1024, generator=gen(seed), device="cuda").bfloat16()
+        weight = torch.randint(-127, 128, (512, 1024), generator=gen(seed + 1), device="cuda", dtype=torch.int8)
+        codes, scale, _ = T.rms_norm_i8(x, x[0].contiguous())
+        q = T.linear_i8(codes, scale, weight, scale.new_full((512,), 1e-3)).view(2, 30, 8, 64)
+        return T.cross_attention(q, q[:, :, :4], q[:, :, 4:])
+
+    def many(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [call(seed) for _ in range(200)]
+            torch.cuda.current_stream().synchronize()
+            return got
+
+    want = [call(seed) for seed in (1, 50)]
+    with ThreadPoolExecutor(2) as pool:
+        for got, one in zip(pool.map(many, (1, 50)), want):
+            assert all(torch.equal(t, one) for t in got)
+    T.check()
