@@ -26,8 +26,13 @@
  *   - It returns 0, -1 (bad argument), SPKV2_ERR_UNSUPPORTED (type or size
  *     outside the ranges below) or a CUDA-target error code
  *     (spkv2_cuda.h).  Calls with nothing to write return 0.
- *   - Sums, norms, softmax statistics and accumulators are fp32 or int32;
- *     a result is rounded once, when it is stored.
+ *   - Sums, norms, softmax statistics and accumulators are fp32 or int32 (fp64
+ *     for the scale of a row whose squares leave fp32's range); a result is
+ *     rounded when it is stored.  Two roundings come before: cross_attention
+ *     rounds each probability to a 16-bit type of its inputs, as both operands
+ *     of a tensor-core product have one type, and adds them up unrounded; codes
+ *     are y times a reciprocal, so a value that lies midway between two codes, to
+ *     2^-14 of a step, may take either.
  *   - Results do not depend on timing: the same call gives the same bits.
  */
 #ifndef SPKV2_TRANSFORMER_H
@@ -146,8 +151,9 @@ typedef struct {
 
 int spkv2_cuda_cross_attention(const Spkv2CrossAttention *args, void *stream);
 
-/* Every wait inside the kernels has a limit of about a second; one that runs
- * out records a role code (2 operand loads, 3 matrix products, 4 results, 7
+/* Every wait for data inside the kernels (on an mbarrier) has a limit of about a
+ * second; the barriers of a cluster and the allocation of tensor memory wait for
+ * CTAs of the GPU only, without one.  A wait that runs out records a role code (2 operand loads, 3 matrix products, 4 results, 7
  * hand-over) on the device and lets its kernel return, with its outputs
  * incomplete.  This call waits for the current device's work and returns 0, or
  * SPKV2_ERR_DEVICE_STATUS with the first such code since the last call. */

@@ -23,7 +23,7 @@
 //
 // With too few row tiles for the SMs the CTAs of a cluster divide the keys, as in
 // the other kernels.  Bound by the MMAs and what splits their operands: 40 TFLOP/s of
-// answers (4 x 1024 x 16 heads, 1024 keys, width 128: 852 us; on CUDA cores 1339 us),
+// answers (4 x 1024 x 16 heads, 1024 keys, width 128: 865 us; on CUDA cores 1339 us),
 // three TF32 MMAs each.
 #include "cross_attention.cuh"
 
@@ -456,8 +456,8 @@ int launch(AttnArgs a, int csize, cudaStream_t s) {
 }
 
 // Warps a row and CTAs a cluster by an estimate of the time in microseconds, fitted
-// to sweeps of both over ten sizes (the choice took at most 25 % longer than the
-// best): a tile takes its warps `wait` + `work` / W one after another, and an SM
+// to sweeps of both over ten sizes (over sixteen, the choice took at most 16 % longer
+// than the best, for thirteen at most 1 %): a tile takes its warps `wait` + `work` / W one after another, and an SM
 // `share` + `full` / W of its throughput; a cluster of eight is slow to start where
 // there are more CTAs than SMs.
 template <int D>

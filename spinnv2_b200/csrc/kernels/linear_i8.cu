@@ -557,9 +557,10 @@ int launch_pair(const LinearArgs &p, const CUtensorMap &ymap, int n_tiles, int m
 }
 
 // The cheapest shape by an estimate of its time in microseconds, fitted to
-// measured sweeps over all shapes of some forty sizes (1 .. 12544 tokens, k 93 ..
-// 16000, n 64 .. 16384; the choice took at most 22 % longer than the best one, over
-// most sizes less than 5 %):
+// measured sweeps over all shapes of some forty sizes (1 .. 16000 tokens, k 93 ..
+// 16384, n 64 .. 16384).  Over 40 sizes the choice was within 5 % of the best shape
+// for 35, within 20 % for 39, and 36 % behind for 6000 x 8000 x 640, where 120 CTAs of
+// 256 columns reach L2's limit, which the estimate sees from the second tile on only:
 //   single tile: 2.6 launch, 0.7 first operands (once where a CTA leaves room
 //     for a second on its SM), 0.2 a K step (0.28 with 256 columns) while every
 //     SM has one tile and 0.0015 a row of operands beyond, when L2 is the limit;

@@ -7,7 +7,8 @@
 // The factor 1 / sqrt(..) is common to a row, so it cancels in the codes:
 //   code = rne(s w * (127 / max|s w|)),  scale = max|s w| / sqrt(..) / 127,
 // and both reductions (sum of s^2, max |s w|) run in one pass over the row.
-// Quantising without the norm is the same with r = 0, w = 1 and no factor.
+// Quantising without the norm is the same with r = 0, w = 1 and no factor.  Rows
+// whose squares leave fp32's range are scaled by a power of two first.
 //
 // The maximum keeps a NaN, so it says by itself whether the row is finite.
 #include "tcgen05.cuh"
@@ -487,8 +488,9 @@ __device__ __noinline__ void wide_row_scaled(RowArgs p, int64_t row, float *s_su
   }
 }
 
-// Rows wider than kMostWidth, the registers of a block: one block a row, which is read twice, the second time from L2; the sum is written in the
-// second pass, as it may take x's or the residual's place.
+// Rows wider than kMostWidth, the registers of a block: one block a row, which is read
+// twice, the second time from L2; the sum is written in the second pass, as it may take
+// x's or the residual's place.
 template <class T, bool NORM>
 __global__ void __launch_bounds__(1024, 2) wide_codes_kernel(RowArgs p) {
   pdl_launch_dependents();

@@ -11,7 +11,9 @@ decoder that reads them needs next to it:
 
 Each call launches on `stream` (a cudaStream_t as an int, or an object with `cuda_stream`; default: torch's
 current stream of the tensors' device) and returns at once.  Outputs are allocated unless they are given.
-Codes that a call allocates start their rows on 16-byte boundaries, whatever the width, which is what
+A tensor used on another stream than its own has to live until that stream is done with it
+(Tensor.record_stream), as in any torch call.  The calls are for inference: what they answer carries no
+gradient, also where an argument requires one.  Codes that a call allocates start their rows on 16-byte boundaries, whatever the width, which is what
 linear_i8 reads fastest.  A wrong type raises TypeError, a wrong shape, device or stride ValueError, and a
 code of the library Spkv2Error.  The checks run in the compiled binding (binding/torch_ops.cpp): a call
 takes about a microsecond more than the launch.
@@ -73,7 +75,7 @@ def linear_i8(codes, scale, weight, weight_scale, *, bias=None, activation=None,
     """act(float(codes @ weight.T) * scale[..., None] * weight_scale + bias), in `dtype` (or out's).
 
     codes [..., k] and weight [n, k] are int8, scale [...], weight_scale [n] and bias [n] float32; the
-    product is exact in 32 bits (k <= 131071).  activation: None, "relu" or "silu".
+    product is exact in 32 bits (k <= 131071).  activation: None, "relu" (which keeps a NaN) or "silu".
     """
     act = _ACTIVATIONS.get(activation)
     if act is None:
@@ -87,7 +89,8 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale: float | None
 
     Key j of entry b counts if j < lengths[b] (int32 [batch]) and key_mask[b, j] (bool or uint8 [batch,
     keys]), where they are given.  What lies in keys and values that do not count has no influence, and a
-    query without keys is answered with zeros.  scale: 1 / sqrt(width) by default.
+    query without keys is answered with zeros.  scale: 1 / sqrt(width) by default.  In 16-bit types each
+    probability is rounded to the type before it meets its value.
     """
     return _ops.cross_attention(q, k, v, lengths, key_mask, scale, out, stream)
 
