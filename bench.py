@@ -233,6 +233,15 @@ def cpu_oracle_int8_throughput(config: str, batch: int, seconds: float, max_step
     return {"value": batch / per, "step_s": per, "steps": len(times), "times": times}
 
 
+def reference_missing() -> str | None:
+    """Why the reference CPU runtime cannot run here, or None."""
+    import oracle
+
+    if oracle.REF_LIB.exists():
+        return None
+    return f"{oracle.REF_LIB.relative_to(REPO)} is not built: it is compiled from the reference's sources, which are not here"
+
+
 def cpu_reference_throughput(config: str, batch: int, seconds: float, max_steps: int | None = None) -> dict:
     """Reference CPU runtime (oracle/_ref) img/s on a bounded sample."""
     from oracle import refrt
@@ -273,6 +282,10 @@ def run_reference_arm(args, group) -> None:
     """The reference CPU runtime on the host cores, on the GPU arm's config
     and batch: every step runs the whole batch (rank 0 only)."""
     if group.rank != 0:
+        return
+    missing = None if args.int8 else reference_missing()
+    if missing:
+        print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
         return
     use_all_host_threads()
     if args.int8:
@@ -649,7 +662,10 @@ def run_gpu_arm(args, group) -> None:
         if strong:
             line["strong"] = strong
         line.update(extras)
-        if world == 1 and not args.no_cpu_baseline:
+        missing = None if args.int8 else reference_missing()
+        if world == 1 and not args.no_cpu_baseline and missing:
+            line["cpu_baseline"] = {"unavailable": missing}
+        elif world == 1 and not args.no_cpu_baseline:
             use_all_host_threads()
             timer = cpu_oracle_int8_throughput if args.int8 else cpu_reference_throughput
             cb = timer(args.config, 1, seconds=args.cpu_seconds)
