@@ -132,7 +132,8 @@ int spkv2_cuda_linear_i8(const Spkv2LinearI8 *args, void *stream);
  * outside 0 .. keys are clamped) and key_mask[b, j] != 0 (where it is given).
  * What lies in the keys and values that do not count has no influence, NaN
  * included.  A row without keys is 0.  heads is a multiple of kv_heads;
- * width: 1 .. 256, the same for keys and values. */
+ * width: 1 .. 256, the same for keys and values.  A stride of 0 stands for one
+ * place for all, in the inputs only. */
 typedef struct {
     const void *q;           /* [batch, queries, heads, width] */
     const void *k;           /* [batch, keys, kv_heads, width] in q's type */

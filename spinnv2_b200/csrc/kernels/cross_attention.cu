@@ -313,6 +313,9 @@ extern "C" int spkv2_cuda_cross_attention(const Spkv2CrossAttention *x, void *st
   if (!x->q || !x->out || (x->keys > 0 && (!x->k || !x->v))) return -1;
   for (int i = 0; i < 3; ++i)
     if (x->q_stride[i] < 0 || x->k_stride[i] < 0 || x->v_stride[i] < 0 || x->out_stride[i] < 0) return -1;
+  const int64_t extent[3] = {x->batch, x->queries, x->heads};
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] > 1 && x->out_stride[i] == 0) return -1;  // one place for several answers
   if (x->key_mask && x->mask_stride < 0) return -1;
   if (!isfinite(x->scale)) return -1;
   const int group = x->heads / x->kv_heads;

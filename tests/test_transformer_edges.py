@@ -395,3 +395,19 @@ def test_calls_from_two_threads(gpu):
         for got, one in zip(pool.map(many, (1, 50)), want):
             assert all(torch.equal(t, one) for t in got)
     T.check()
+
+
+# ------------------------------------------------------------------ refusals
+def test_answers_in_one_place_are_refused(built):
+    """A stride of 0 between answers is a bad argument, before any CUDA call; of a dimension of one it is none."""
+    from test_transformer import CROSS, c_function
+
+    fake = 4096  # never read
+    base = dict(q=fake, k=fake, v=fake, o=fake, l=0, m=0, b=2, lq=3, lk=1)
+    base.update({f"st{i}": 8 for i in range(12)}, ms=0, h=2, hk=1, d=300, t=1, sc=1.0, r=0)  # too wide: no launch
+    for i in (9, 10, 11):
+        assert c_function("spkv2_cuda_cross_attention")(CROSS.pack(*{**base, f"st{i}": 0}.values()), None) == -1
+        one = {**base, f"st{i}": 0, "b": 1, "lq": 1, "h": 1}
+        assert c_function("spkv2_cuda_cross_attention")(CROSS.pack(*one.values()), None) == -43
+    for i in range(9):  # inputs may
+        assert c_function("spkv2_cuda_cross_attention")(CROSS.pack(*{**base, f"st{i}": 0}.values()), None) == -43
